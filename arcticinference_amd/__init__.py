@@ -9,6 +9,8 @@ __version__ = "0.1.0"
 from . import py_custom_ops  # noqa: F401
 from .py_custom_ops import (  # noqa: F401
     gather_rows,
+    paged_attention,
+    paged_attention_ragged,
     reshape_and_cache_flash_bulk,
     reshape_and_cache_flash_bulk_select,
     reshape_and_cache_flash_fp4,
@@ -23,4 +25,5 @@ from .py_custom_ops import (  # noqa: F401
     sum_lstm_shared_z,
     try_load_jit_library,
     try_load_torch_library,
+    verify_draft_tokens,
 )

@@ -40,7 +40,25 @@ EXPORTED_SYMBOLS = (
     "arctic_argmax_clamp_split",
     "arctic_argmax_workspace_bytes",
     "arctic_argmax_workspace_bytes_at",
+    "arctic_paged_attention",
+    "arctic_paged_attention_workspace_bytes",
+    "arctic_paged_attention_ragged",
+    "arctic_paged_attention_ragged_workspace_bytes",
+    "arctic_verify_drafts",
+    "arctic_verify_drafts_workspace_bytes",
 )
+
+
+
+class PagedCache(ctypes.Structure):
+    """``arctic_paged_cache`` of include/arctic_mi355x.h."""
+    _fields_ = [("key_cache", ctypes.c_void_p), ("value_cache", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("num_blocks", ctypes.c_int64), ("key_block_stride", ctypes.c_int64),
+                ("key_token_stride", ctypes.c_int64), ("key_head_stride", ctypes.c_int64),
+                ("value_block_stride", ctypes.c_int64), ("value_token_stride", ctypes.c_int64),
+                ("value_head_stride", ctypes.c_int64), ("block_size", ctypes.c_int), ("num_kv_heads", ctypes.c_int),
+                ("head_size", ctypes.c_int), ("kv_cache_dtype", ctypes.c_int)]
+
 
 _lib: Optional[ctypes.CDLL] = None
 
@@ -123,6 +141,23 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.arctic_argmax_workspace_bytes.restype = i64
     lib.arctic_argmax_workspace_bytes_at.argtypes = [vp, i64, i32, i64, i32]
     lib.arctic_argmax_workspace_bytes_at.restype = i64
+    cache = ctypes.POINTER(PagedCache)
+    lib.arctic_paged_attention_workspace_bytes.argtypes = [i64, i32, i32, cache, i64, i64, i64, i32]
+    lib.arctic_paged_attention_workspace_bytes.restype = i64
+    lib.arctic_paged_attention.argtypes = [
+        vp, vp, cache, vp, vp, i64, i32, i32, i64, i64,   # out ... seq_lens, batch, new_tokens, num_heads, the table's sizes
+        i64, i64, i64, i64, f32, i64, i64, i64, i32,      # pitches, scale, max_seq_len, window, num_sinks, dtype
+        vp, i64, vp]                                      # workspace, its bytes, stream
+    lib.arctic_paged_attention.restype = i32
+    lib.arctic_paged_attention_ragged_workspace_bytes.argtypes = [i64, i64, i32, cache, i64, i64, i64, i32]
+    lib.arctic_paged_attention_ragged_workspace_bytes.restype = i64
+    lib.arctic_paged_attention_ragged.argtypes = [
+        vp, vp, vp, cache, vp, vp, i64, i64, i32, i64, i64, i64, i64, i64, i64, f32, i64, i64, i64, i32, vp, i64, vp]
+    lib.arctic_paged_attention_ragged.restype = i32
+    lib.arctic_verify_drafts_workspace_bytes.argtypes = [i64, i32, i32, i32]
+    lib.arctic_verify_drafts_workspace_bytes.restype = i64
+    lib.arctic_verify_drafts.argtypes = [vp] * 8 + [i64, i32, i64, i32, i64, i64, i64, i32, vp, i64, vp]
+    lib.arctic_verify_drafts.restype = i32
 
 
 def load() -> ctypes.CDLL:

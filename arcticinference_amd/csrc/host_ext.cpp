@@ -330,6 +330,26 @@ at::Tensor speculator_argmax_cuda(const at::Tensor &logits, int64_t max_index) {
   return arctic_host::argmax_clamp(logits, max_index);
 }
 
+void paged_attention(const at::Tensor &query, const at::Tensor &key_cache, const at::Tensor &value_cache,
+                     const at::Tensor &block_table, const at::Tensor &seq_lens, const std::string &kv_cache_dtype,
+                     const at::Tensor &k_scale, const at::Tensor &v_scale, double scale, int64_t max_seq_len, int64_t window,
+                     int64_t num_sinks, const at::Tensor &out) {
+  arctic_host::paged_attention(query, c10::nullopt, key_cache, value_cache, block_table, seq_lens, kv_cache_dtype, k_scale,
+                               v_scale, scale, max_seq_len, window, num_sinks, out);
+}
+void paged_attention_ragged(const at::Tensor &query, const at::Tensor &query_start, const at::Tensor &key_cache,
+                            const at::Tensor &value_cache, const at::Tensor &block_table, const at::Tensor &seq_lens,
+                            const std::string &kv_cache_dtype, const at::Tensor &k_scale, const at::Tensor &v_scale,
+                            double scale, int64_t max_seq_len, int64_t window, int64_t num_sinks, const at::Tensor &out) {
+  arctic_host::paged_attention(query, query_start, key_cache, value_cache, block_table, seq_lens, kv_cache_dtype, k_scale,
+                               v_scale, scale, max_seq_len, window, num_sinks, out);
+}
+TwoTensors verify_draft_tokens(const at::Tensor &logits, const at::Tensor &row_start, const at::Tensor &draft_token_ids,
+                               const at::Tensor &accept_uniforms, const at::Tensor &sample_uniforms,
+                               const OptTensor &temperatures) {
+  return arctic_host::verify_drafts(logits, row_start, draft_token_ids, accept_uniforms, sample_uniforms, temperatures);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host_ext, m) {
@@ -347,6 +367,9 @@ PYBIND11_MODULE(_host_ext, m) {
   def<&gather_rows>(m, "gather_rows");
   def<&scatter_rows>(m, "scatter_rows");
   def<&speculator_argmax_cuda>(m, "speculator_argmax_cuda");
+  def<&paged_attention>(m, "paged_attention");
+  def<&paged_attention_ragged>(m, "paged_attention_ragged");
+  def<&verify_draft_tokens>(m, "verify_draft_tokens");
   static PyMethodDef method = {"on_gpu", on_gpu, METH_O, nullptr};
   m.add_object("on_gpu", py::reinterpret_steal<py::object>(PyCFunction_New(&method, nullptr)));
   py::class_<PreparedLayers>(m, "BulkKVLayers")

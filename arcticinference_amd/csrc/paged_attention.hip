@@ -1,0 +1,262 @@
+// Attention of new tokens over a paged key-value cache, gfx950.
+//
+// The caches are the ones that reshape_and_cache_flash_bulk writes.  Sequence b has L tokens in them, its n queries are
+// the last n; the query at position p sees the keys j <= p that lie in its window (j > p - window) or among the first
+// `sinks` tokens:
+//   s_j = scale k_scale <q, K_j>,   out = v_scale sum_j exp(s_j - m) V_j / sum_j exp(s_j - m),   m = max_j s_j
+// A query that sees nothing answers zeros.  A page outside the cache holds no keys.
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "paged_attention.hpp"
+
+namespace arctic {
+
+// Any head size up to 512, any type, alignment and stride: one wave per query and head.  64 keys at a time: every lane
+// takes the product of one key with the query, the running maximum and sum are the wave's, then every lane adds the
+// weighted values of its elements, key by key.  A key that is not seen is not read, so what it holds does not matter.
+constexpr int kGeneralMostHead = 512;
+
+template <typename Q, typename C>
+__global__ __launch_bounds__(64) void attention_general_kernel(const AttentionParams p) {
+  __shared__ float query[kGeneralMostHead];
+  __shared__ float weight[64];
+  __shared__ int64_t value_at[64];
+  const int lane = threadIdx.x;
+  const uint32_t token = p.by_heads.quotient(blockIdx.x);
+  const int head = (int)(blockIdx.x - token * (uint32_t)p.heads);
+  int b, count, first;
+  if (p.query_start) {
+    int lo = 0, hi = p.batch;   // the last sequence that starts at or before this row
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (p.query_start[mid] <= (int)token) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+    first = p.query_start[b];
+    count = p.query_start[b + 1] - first;
+    if (first < 0 || (int)token < first || (int)token - first >= count) return;   // a row of no sequence
+  } else {
+    b = (int)p.by_new.quotient(token);
+    first = b * p.new_tokens;
+    count = p.new_tokens;
+  }
+  const int position = clamped_length(p, b) - count + ((int)token - first);
+  const int kv_head = (int)p.by_group.quotient((uint32_t)head);
+  const int D = p.head_size;
+  const char *q = p.query + (int64_t)token * p.query_token + (int64_t)head * p.query_head;
+  for (int d = lane; d < D; d += 64) query[d] = Q::load(q + (int64_t)d * Q::kBytes);
+  __syncthreads();
+  const float scale = p.scale * (p.k_scale ? *p.k_scale : 1.f);
+  const int start = window_start(p, position);
+  const int sinks = min(p.sinks, start);
+  const int keys = position < 0 ? 0 : sinks + (position - start + 1);
+  float acc[kGeneralMostHead / 64] = {};
+  float m = -__builtin_inff(), sum = 0.f;
+  for (int k0 = 0; k0 < keys; k0 += 64) {
+    const int k = k0 + lane;
+    float s = -__builtin_inff();
+    int64_t at = -1;
+    if (k < keys) {
+      const int j = k < sinks ? k : start + (k - sinks);
+      const int block = (int)p.by_block.quotient((uint32_t)j);
+      const int64_t page = p.table[(int64_t)b * p.table_row + block];
+      if (page >= 0 && page < p.num_blocks) {
+        const int off = j - block * p.block_size;
+        const char *key = p.key_cache + page * p.key_block + (int64_t)off * p.key_token + (int64_t)kv_head * p.key_head;
+        at = page * p.value_block + (int64_t)off * p.value_token + (int64_t)kv_head * p.value_head;
+        float dot = 0.f;
+        for (int d = 0; d < D; ++d) dot = fmaf(query[d], C::load(key + (int64_t)d * C::kBytes), dot);
+        s = dot * scale;
+      }
+    }
+    const bool nan = __any(s != s);
+    const float top = nan ? __builtin_nanf("") : fmaxf(m, wave_max(s));
+    const float base = top == -__builtin_inff() ? 0.f : top;
+    const float w = at < 0 ? 0.f : __expf(s - base);
+    const float keep = __expf(m - base);
+    __syncthreads();
+    weight[lane] = w;
+    value_at[lane] = at;
+    __syncthreads();
+    float chunk = w;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) chunk += __shfl_xor(chunk, d);
+    sum = sum * keep + chunk;
+    m = top;
+#pragma unroll
+    for (int i = 0; i < kGeneralMostHead / 64; ++i) acc[i] *= keep;
+    const int n = min(64, keys - k0);
+    for (int k = 0; k < n; ++k) {
+      if (value_at[k] < 0) continue;
+      const char *value = p.value_cache + value_at[k] + (int64_t)lane * C::kBytes;
+#pragma unroll
+      for (int i = 0; i < kGeneralMostHead / 64; ++i)
+        if (lane + 64 * i < D) acc[i] = fmaf(weight[k], C::load(value + 64 * i * C::kBytes), acc[i]);
+    }
+  }
+  const float norm = sum == 0.f ? 0.f : (p.v_scale ? *p.v_scale : 1.f) / sum;
+  char *out = p.out + (int64_t)token * p.out_token + (int64_t)head * p.out_head;
+#pragma unroll
+  for (int i = 0; i < kGeneralMostHead / 64; ++i)
+    if (lane + 64 * i < D) Q::store(out + (int64_t)(lane + 64 * i) * Q::kBytes, acc[i] * norm);
+}
+
+}  // namespace arctic
+
+using namespace arctic;
+
+// The checks that both entry points share, and the call's description for the kernels.
+static int describe(const char *fn, AttentionParams &p, void *out, const void *query, const arctic_paged_cache *cache,
+                    const int32_t *block_table, const int32_t *seq_lens, int64_t batch, int64_t max_blocks,
+                    int64_t table_stride, int64_t total_tokens, int num_heads, int64_t query_token_stride,
+                    int64_t query_head_stride, int64_t out_token_stride, int64_t out_head_stride, float scale,
+                    int64_t window, int64_t num_sinks, int dtype) {
+  if (dtype != ARCTIC_DTYPE_F32 && dtype != ARCTIC_DTYPE_F16 && dtype != ARCTIC_DTYPE_BF16)
+    return fail(ARCTIC_ERR_UNSUPPORTED, "%s: queries must be fp32, fp16 or bf16", fn);
+  if (!cache) return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: null cache description", fn);
+  const arctic_paged_cache &c = *cache;
+  if (c.kv_cache_dtype != ARCTIC_KV_AUTO && c.kv_cache_dtype != ARCTIC_KV_FP8_E4M3 && c.kv_cache_dtype != ARCTIC_KV_FP8_E5M2)
+    return fail(ARCTIC_ERR_UNSUPPORTED, "%s: Unsupported data type of kv cache: code %d", fn, c.kv_cache_dtype);
+  if (batch < 0 || total_tokens < 0 || num_heads <= 0 || c.num_kv_heads <= 0 || c.head_size <= 0 || c.block_size <= 0 ||
+      max_blocks < 0 || c.num_blocks < 0)
+    return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: sizes must be positive", fn);
+  if (num_heads % c.num_kv_heads)
+    return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: num_heads (%d) must be a multiple of num_kv_heads (%d)", fn, num_heads,
+                c.num_kv_heads);
+  if (c.head_size > kGeneralMostHead)
+    return fail(ARCTIC_ERR_UNSUPPORTED, "%s: head_size must be at most %d", fn, kGeneralMostHead);
+  if (batch > 0x7ffffffeLL || total_tokens > 0x7fffffffLL || num_heads > (1 << 20) || c.block_size > (1 << 20) ||
+      c.num_blocks > ((int64_t)1 << 31) || max_blocks > 0x7fffffffLL || total_tokens * num_heads > 0x7fffffffLL)
+    return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: batch, tokens, tokens * num_heads, max_blocks or num_blocks beyond 2^31, "
+                "num_heads or block_size beyond 2^20", fn);
+  if (window < 0 || num_sinks < 0)
+    return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: window and num_sinks must not be negative", fn);
+  const int es = dtype == ARCTIC_DTYPE_F32 ? 4 : 2, cs = c.kv_cache_dtype == ARCTIC_KV_AUTO ? es : 1;
+  if (!pitch_ok(query_token_stride, total_tokens, es) || !pitch_ok(query_head_stride, num_heads, es) ||
+      !pitch_ok(out_token_stride, total_tokens, es) || !pitch_ok(out_head_stride, num_heads, es) ||
+      !pitch_ok(c.key_block_stride, c.num_blocks, cs) || !pitch_ok(c.key_token_stride, c.block_size, cs) ||
+      !pitch_ok(c.key_head_stride, c.num_kv_heads, cs) || !pitch_ok(c.value_block_stride, c.num_blocks, cs) ||
+      !pitch_ok(c.value_token_stride, c.block_size, cs) || !pitch_ok(c.value_head_stride, c.num_kv_heads, cs) ||
+      !pitch_ok(table_stride, batch, 4))
+    return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: query, output, cache or table pitch out of range", fn);
+  if (batch == 0 || total_tokens == 0) return ARCTIC_OK;
+  if (!out || !query || !seq_lens || (max_blocks > 0 && !block_table) || (c.num_blocks > 0 && (!c.key_cache || !c.value_cache)))
+    return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: null tensor pointer", fn);
+  if (c.kv_cache_dtype != ARCTIC_KV_AUTO && (!c.k_scale || !c.v_scale))
+    return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: an fp8 cache needs k_scale and v_scale", fn);
+  if (((uintptr_t)out | (uintptr_t)query) % es ||
+      ((uintptr_t)c.key_cache | (uintptr_t)c.value_cache) % cs || ((uintptr_t)block_table | (uintptr_t)seq_lens) % 4)
+    return fail(ARCTIC_ERR_UNSUPPORTED, "%s: a tensor does not start at a multiple of its element size", fn);
+  const bool quantised = c.kv_cache_dtype != ARCTIC_KV_AUTO;
+  p.query = (const char *)query;
+  p.out = (char *)out;
+  p.key_cache = (const char *)c.key_cache;
+  p.value_cache = (const char *)c.value_cache;
+  p.table = block_table;
+  p.seq_lens = seq_lens;
+  p.query_start = nullptr;
+  p.k_scale = quantised ? c.k_scale : nullptr;
+  p.v_scale = quantised ? c.v_scale : nullptr;
+  p.query_token = query_token_stride * es;
+  p.query_head = query_head_stride * es;
+  p.out_token = out_token_stride * es;
+  p.out_head = out_head_stride * es;
+  p.key_block = c.key_block_stride * cs;
+  p.key_token = c.key_token_stride * cs;
+  p.key_head = c.key_head_stride * cs;
+  p.value_block = c.value_block_stride * cs;
+  p.value_token = c.value_token_stride * cs;
+  p.value_head = c.value_head_stride * cs;
+  p.table_row = table_stride;
+  p.num_blocks = c.num_blocks;
+  p.total_tokens = total_tokens;
+  p.batch = (int)batch;
+  p.new_tokens = 0;
+  p.max_blocks = (int)max_blocks;
+  p.block_size = c.block_size;
+  p.heads = num_heads;
+  p.kv_heads = c.num_kv_heads;
+  p.group = num_heads / c.num_kv_heads;
+  p.head_size = c.head_size;
+  p.window = (int)(window > 0x7fffffffLL ? 0 : window);   // every position is below 2^31
+  p.sinks = (int)(num_sinks > 0x7fffffffLL ? 0x7fffffffLL : num_sinks);
+  p.scale = scale;
+  p.by_block = Divisor((uint32_t)c.block_size);
+  p.by_group = Divisor((uint32_t)p.group);
+  p.by_heads = Divisor((uint32_t)num_heads);
+  p.by_new = Divisor(1);
+  return ARCTIC_OK;
+}
+
+template <typename Q>
+static void launch_general(const AttentionParams &p, int kv, hipStream_t s) {
+  const dim3 grid((unsigned)(p.total_tokens * p.heads));
+  if (kv == ARCTIC_KV_AUTO) launch(attention_general_kernel<Q, Q>, grid, 64, s, p);
+  else if (kv == ARCTIC_KV_FP8_E4M3) launch(attention_general_kernel<Q, CacheE4M3>, grid, 64, s, p);
+  else launch(attention_general_kernel<Q, CacheE5M2>, grid, 64, s, p);
+}
+
+static int run_attention(const char *fn, const AttentionParams &p, int dtype, int kv, hipStream_t s) {
+  if (dtype == ARCTIC_DTYPE_F32) launch_general<F32>(p, kv, s);
+  else if (dtype == ARCTIC_DTYPE_F16) launch_general<Half<F16>>(p, kv, s);
+  else launch_general<Half<BF16>>(p, kv, s);
+  return check_launch(fn);
+}
+
+extern "C" int64_t arctic_paged_attention_workspace_bytes(int64_t batch, int new_tokens, int num_heads,
+                                                          const arctic_paged_cache *cache, int64_t max_seq_len,
+                                                          int64_t window, int64_t num_sinks, int dtype) {
+  (void)batch, (void)new_tokens, (void)num_heads, (void)cache, (void)max_seq_len, (void)window, (void)num_sinks, (void)dtype;
+  return 0;
+}
+
+extern "C" int arctic_paged_attention(void *out, const void *query, const arctic_paged_cache *cache,
+                                      const int32_t *block_table, const int32_t *seq_lens, int64_t batch, int new_tokens,
+                                      int num_heads, int64_t max_blocks, int64_t table_stride,
+                                      int64_t query_token_stride, int64_t query_head_stride, int64_t out_token_stride,
+                                      int64_t out_head_stride, float scale, int64_t max_seq_len, int64_t window,
+                                      int64_t num_sinks, int dtype, void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *fn = "paged_attention";
+  if (new_tokens < 0 || batch < 0 || (new_tokens > 0 && batch > 0x7fffffffLL / new_tokens))
+    return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: batch and new_tokens must not be negative, nor their product beyond 2^31", fn);
+  AttentionParams p;
+  const int rc = describe(fn, p, out, query, cache, block_table, seq_lens, batch, max_blocks, table_stride, batch * new_tokens,
+                          num_heads, query_token_stride, query_head_stride, out_token_stride, out_head_stride, scale, window,
+                          num_sinks, dtype);
+  if (rc != ARCTIC_OK || batch == 0 || new_tokens == 0) return rc;
+  (void)max_seq_len, (void)workspace, (void)workspace_bytes;
+  p.new_tokens = new_tokens;
+  p.by_new = Divisor((uint32_t)new_tokens);
+  return run_attention(fn, p, dtype, cache->kv_cache_dtype, (hipStream_t)stream);
+}
+
+extern "C" int64_t arctic_paged_attention_ragged_workspace_bytes(int64_t batch, int64_t total_tokens, int num_heads,
+                                                                 const arctic_paged_cache *cache, int64_t max_seq_len,
+                                                                 int64_t window, int64_t num_sinks, int dtype) {
+  (void)batch, (void)total_tokens, (void)num_heads, (void)cache, (void)max_seq_len, (void)window, (void)num_sinks, (void)dtype;
+  return 0;
+}
+
+extern "C" int arctic_paged_attention_ragged(void *out, const void *query, const int32_t *query_start,
+                                             const arctic_paged_cache *cache, const int32_t *block_table,
+                                             const int32_t *seq_lens, int64_t batch, int64_t total_tokens, int num_heads,
+                                             int64_t max_blocks, int64_t table_stride, int64_t query_token_stride,
+                                             int64_t query_head_stride, int64_t out_token_stride, int64_t out_head_stride,
+                                             float scale, int64_t max_seq_len, int64_t window, int64_t num_sinks, int dtype,
+                                             void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *fn = "paged_attention_ragged";
+  AttentionParams p;
+  const int rc = describe(fn, p, out, query, cache, block_table, seq_lens, batch, max_blocks, table_stride, total_tokens,
+                          num_heads, query_token_stride, query_head_stride, out_token_stride, out_head_stride, scale, window,
+                          num_sinks, dtype);
+  if (rc != ARCTIC_OK || batch == 0 || total_tokens == 0) return rc;
+  if (!query_start || (uintptr_t)query_start % 4)
+    return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: query_start is missing or not aligned", fn);
+  (void)max_seq_len, (void)workspace, (void)workspace_bytes;
+  p.query_start = query_start;
+  return run_attention(fn, p, dtype, cache->kv_cache_dtype, (hipStream_t)stream);
+}

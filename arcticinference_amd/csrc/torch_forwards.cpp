@@ -81,6 +81,15 @@ bool is_half(const at::Tensor &t) { return t.scalar_type() == at::kHalf || t.sca
 
 int half_code(const at::Tensor &t) { return t.scalar_type() == at::kHalf ? ARCTIC_DTYPE_F16 : ARCTIC_DTYPE_BF16; }
 
+int float_code(const at::Tensor &t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return ARCTIC_DTYPE_F32;
+    case at::kHalf: return ARCTIC_DTYPE_F16;
+    case at::kBFloat16: return ARCTIC_DTYPE_BF16;
+    default: return -1;
+  }
+}
+
 // t.view(-1, cols); a tensor that is 2-D already is passed through.  A single row still goes through view(), which
 // sets its row stride to `cols` as the reference's view() does.
 at::Tensor rows_of(const at::Tensor &t, int64_t cols) {
@@ -549,13 +558,7 @@ void move_rows(const char *fn, const TensorList &sources, const at::Tensor &indi
 
 at::Tensor argmax_clamp(const at::Tensor &logits, int64_t max_index) {
   TORCH_CHECK(logits.is_cuda(), "speculator_argmax: logits must be CUDA");
-  int code = -1;
-  switch (logits.scalar_type()) {
-    case at::kFloat: code = ARCTIC_DTYPE_F32; break;
-    case at::kHalf: code = ARCTIC_DTYPE_F16; break;
-    case at::kBFloat16: code = ARCTIC_DTYPE_BF16; break;
-    default: break;
-  }
+  const int code = float_code(logits);
   TORCH_CHECK(code >= 0, "speculator_argmax: logits must be fp32, fp16 or bf16");
   TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) > 0, "speculator_argmax: logits need a non-empty last dimension");
   TORCH_CHECK(logits.stride(-1) == 1, "speculator_argmax: last dimension must be contiguous");
@@ -578,6 +581,160 @@ at::Tensor argmax_clamp(const at::Tensor &logits, int64_t max_index) {
     out.storage().set_nbytes((size_t)rows * sizeof(int64_t));
   }
   return out;
+}
+
+// ---- the operators that read the caches, and the verification of drafts -----------------------------------------
+namespace {
+
+bool int_vector(const at::Tensor &t, int64_t n) {
+  return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && (n <= 1 || t.stride(0) == 1);
+}
+
+}  // namespace
+
+void paged_attention(const at::Tensor &query, const OptTensor &query_start, const at::Tensor &key_cache,
+                     const at::Tensor &value_cache, const at::Tensor &block_table, const at::Tensor &seq_lens,
+                     const std::string &kv_cache_dtype, const at::Tensor &k_scale, const at::Tensor &v_scale, double scale,
+                     int64_t max_seq_len, int64_t window, int64_t num_sinks, const at::Tensor &out) {
+  const bool ragged = given(query_start);
+  const char *fn = ragged ? "paged_attention_ragged" : "paged_attention";
+  const int code = float_code(query);
+  TORCH_CHECK(code >= 0, fn, ": queries must be fp32, fp16 or bf16");
+  int kv = -1;
+  if (kv_cache_dtype == "auto") kv = ARCTIC_KV_AUTO;
+  else if (kv_cache_dtype == "fp8" || kv_cache_dtype == "fp8_e4m3") kv = ARCTIC_KV_FP8_E4M3;
+  else if (kv_cache_dtype == "fp8_e5m2") kv = ARCTIC_KV_FP8_E5M2;
+  TORCH_CHECK(kv >= 0, "Unsupported data type of kv cache: ", kv_cache_dtype);
+  TORCH_CHECK(query.dim() == 3 || (!ragged && query.dim() == 4), fn, ragged ? ": queries must be [tokens, heads, head_size]"
+              : ": queries must be [batch, heads, head_size] or [batch, new tokens, heads, head_size]");
+  TORCH_CHECK(key_cache.dim() == 4 && value_cache.dim() == 4 && key_cache.sizes() == value_cache.sizes(), fn,
+              ": key and value caches must be [blocks, block_size, kv_heads, head_size], both of one shape");
+  const int64_t d = query.dim(), heads = query.size(d - 2), head_size = query.size(d - 1), kv_heads = key_cache.size(2);
+  TORCH_CHECK(head_size >= 1 && key_cache.size(3) == head_size, fn, ": queries and caches differ in their head_size");
+  TORCH_CHECK(heads >= 1 && kv_heads >= 1 && heads % kv_heads == 0, fn, ": the number of heads (", heads,
+              ") must be a multiple of the caches' (", kv_heads, ")");
+  TORCH_CHECK(key_cache.size(1) >= 1, fn, ": block_size must be positive");
+  if (kv == ARCTIC_KV_AUTO) {
+    TORCH_CHECK(key_cache.scalar_type() == query.scalar_type() && value_cache.scalar_type() == query.scalar_type(), fn,
+                ": caches of kv_cache_dtype 'auto' must be of the queries' type");
+  } else {
+    TORCH_CHECK(key_cache.element_size() == 1 && value_cache.element_size() == 1, fn, ": caches of kv_cache_dtype '",
+                kv_cache_dtype, "' must have elements of one byte");
+    TORCH_CHECK(k_scale.scalar_type() == at::kFloat && v_scale.scalar_type() == at::kFloat && k_scale.numel() == 1 &&
+                    v_scale.numel() == 1,
+                fn, ": k_scale and v_scale must be float32 tensors of one element");
+  }
+  TORCH_CHECK(query.stride(d - 1) == 1 || head_size == 1, fn, ": the last dimension of the queries must be contiguous");
+  TORCH_CHECK((key_cache.stride(3) == 1 && value_cache.stride(3) == 1) || head_size == 1, fn,
+              ": the last dimension of the caches must be contiguous");
+  TORCH_CHECK(out.scalar_type() == query.scalar_type() && out.sizes() == query.sizes(), fn,
+              ": out must have the queries' type and shape");
+  TORCH_CHECK(out.stride(d - 1) == 1 || head_size == 1, fn, ": the last dimension of out must be contiguous");
+  const int64_t batch = ragged ? seq_lens.numel() : query.size(0), new_tokens = d == 4 ? query.size(1) : 1;
+  TORCH_CHECK(int_vector(seq_lens, batch), fn, ": seq_lens must be a contiguous int32 tensor with one entry per sequence");
+  TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == batch &&
+                  (block_table.size(1) <= 1 || block_table.stride(1) == 1),
+              fn, ": block_table must be int32 [", batch, ", blocks] with contiguous rows");
+  if (ragged)
+    TORCH_CHECK(int_vector(*query_start, batch + 1), fn, ": query_start must be a contiguous int32 tensor with one entry more than seq_lens");
+  TORCH_CHECK(max_seq_len >= 0, fn, ": max_seq_len must not be negative");
+  TORCH_CHECK(window >= 0 && num_sinks >= 0, fn, ": window must be positive and num_sinks not negative");
+  TORCH_CHECK(query.is_cuda(), fn, ": the tensors must be CUDA tensors");
+  for (const at::Tensor *t : {&key_cache, &value_cache, &block_table, &seq_lens, &out})
+    TORCH_CHECK(t->device() == query.device(), fn, ": all tensors must be on the same device");
+  if (kv != ARCTIC_KV_AUTO)
+    TORCH_CHECK(k_scale.device() == query.device() && v_scale.device() == query.device(), fn,
+                ": all tensors must be on the same device");
+  if (ragged) TORCH_CHECK(query_start->device() == query.device(), fn, ": all tensors must be on the same device");
+  // token b * new_tokens + i of a [batch, new tokens, heads, head_size] tensor lies that many pitches from the first
+  const auto token_pitch = [&](const at::Tensor &t, const char *name) {
+    if (d == 3) return t.stride(0);
+    TORCH_CHECK(batch <= 1 || new_tokens <= 1 || t.stride(0) == new_tokens * t.stride(1), fn, ": the tokens of ", name,
+                " must be one pitch apart");
+    return new_tokens == 1 ? t.stride(0) : t.stride(1);
+  };
+  const int64_t query_token = token_pitch(query, "the queries"), out_token = token_pitch(out, "out");
+  if (query.numel() == 0 || batch == 0) return;
+
+  arctic_paged_cache cache;
+  cache.key_cache = key_cache.data_ptr();
+  cache.value_cache = value_cache.data_ptr();
+  cache.k_scale = kv == ARCTIC_KV_AUTO ? nullptr : (const float *)k_scale.data_ptr();
+  cache.v_scale = kv == ARCTIC_KV_AUTO ? nullptr : (const float *)v_scale.data_ptr();
+  cache.num_blocks = key_cache.size(0);
+  cache.key_block_stride = key_cache.stride(0);
+  cache.key_token_stride = key_cache.stride(1);
+  cache.key_head_stride = key_cache.stride(2);
+  cache.value_block_stride = value_cache.stride(0);
+  cache.value_token_stride = value_cache.stride(1);
+  cache.value_head_stride = value_cache.stride(2);
+  cache.block_size = to_int(key_cache.size(1), "block_size");
+  cache.num_kv_heads = to_int(kv_heads, "kv_heads");
+  cache.head_size = to_int(head_size, "head_size");
+  cache.kv_cache_dtype = kv;
+  const int num_heads = to_int(heads, "heads");
+  const OnDevice device(query);
+  const int64_t bytes =
+      ragged ? arctic_paged_attention_ragged_workspace_bytes(batch, query.size(0), num_heads, &cache, max_seq_len, window,
+                                                             num_sinks, code)
+             : arctic_paged_attention_workspace_bytes(batch, to_int(new_tokens, "new tokens"), num_heads, &cache, max_seq_len,
+                                                      window, num_sinks, code);
+  const at::Tensor workspace = bytes ? new_empty({(bytes + 3) / 4}, at::kFloat, query) : at::Tensor();
+  void *const at_workspace = bytes ? workspace.data_ptr() : nullptr;
+  if (ragged) {
+    check_rc(arctic_paged_attention_ragged(
+        out.data_ptr(), query.data_ptr(), (const int32_t *)query_start->data_ptr(), &cache,
+        (const int32_t *)block_table.data_ptr(), (const int32_t *)seq_lens.data_ptr(), batch, query.size(0), num_heads,
+        block_table.size(1), block_table.stride(0), query_token, query.stride(d - 2), out_token, out.stride(d - 2),
+        (float)scale, max_seq_len, window, num_sinks, code, at_workspace, bytes, device.stream()));
+  } else {
+    check_rc(arctic_paged_attention(
+        out.data_ptr(), query.data_ptr(), &cache, (const int32_t *)block_table.data_ptr(),
+        (const int32_t *)seq_lens.data_ptr(), batch, (int)new_tokens, num_heads, block_table.size(1), block_table.stride(0),
+        query_token, query.stride(d - 2), out_token, out.stride(d - 2), (float)scale, max_seq_len, window, num_sinks, code,
+        at_workspace, bytes, device.stream()));
+  }
+}
+
+std::tuple<at::Tensor, at::Tensor> verify_drafts(const at::Tensor &logits, const at::Tensor &row_start,
+                                                 const at::Tensor &drafts, const at::Tensor &accept_uniforms,
+                                                 const at::Tensor &sample_uniforms, const OptTensor &temperatures) {
+  const char *fn = "verify_draft_tokens";
+  const int code = float_code(logits);
+  TORCH_CHECK(code >= 0, fn, ": logits must be fp32, fp16 or bf16");
+  TORCH_CHECK(logits.dim() == 2 && logits.size(1) > 0, fn, ": logits must be [rows, vocab_size]");
+  TORCH_CHECK(logits.stride(1) == 1 || logits.size(1) == 1, fn, ": rows of logits must be contiguous");
+  TORCH_CHECK(drafts.dim() == 2 && drafts.scalar_type() == at::kLong, fn, ": draft_token_ids must be int64 [batch, drafts]");
+  const int64_t batch = drafts.size(0), most = drafts.size(1);
+  TORCH_CHECK(most <= 1 || drafts.stride(1) == 1, fn, ": rows of draft_token_ids must be contiguous");
+  TORCH_CHECK(int_vector(row_start, batch + 1), fn,
+              ": row_start must be a contiguous int32 tensor with one entry more than there are requests");
+  TORCH_CHECK(accept_uniforms.scalar_type() == at::kFloat && accept_uniforms.sizes() == drafts.sizes() &&
+                  (most <= 1 || accept_uniforms.stride(1) == 1),
+              fn, ": accept_uniforms must be float32, of draft_token_ids' shape, with contiguous rows");
+  const auto per_request = [&](const at::Tensor &t, const char *name) {
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == batch && (batch <= 1 || t.stride(0) == 1), fn, ": ",
+                name, " must be a contiguous float32 tensor with one entry per request");
+  };
+  per_request(sample_uniforms, "sample_uniforms");
+  if (given(temperatures)) per_request(*temperatures, "temperatures");
+  TORCH_CHECK(logits.is_cuda(), fn, ": the tensors must be CUDA tensors");
+  for (const at::Tensor *t : {&row_start, &drafts, &accept_uniforms, &sample_uniforms})
+    TORCH_CHECK(t->device() == logits.device(), fn, ": all tensors must be on the same device");
+  if (given(temperatures)) TORCH_CHECK(temperatures->device() == logits.device(), fn, ": all tensors must be on the same device");
+  const int max_drafts = to_int(most, "drafts"), vocab = to_int(logits.size(1), "vocab_size");
+  const OnDevice device(logits);
+  const at::Tensor tokens = new_empty({batch, most + 1}, at::kLong, logits), counts = new_empty({batch}, at::kLong, logits);
+  if (batch == 0) return std::make_tuple(tokens, counts);
+  const int64_t bytes = arctic_verify_drafts_workspace_bytes(batch, max_drafts, vocab, code);
+  const at::Tensor workspace = new_empty({(bytes + 7) / 8}, at::kLong, logits);
+  check_rc(arctic_verify_drafts((int64_t *)tokens.data_ptr(), (int64_t *)counts.data_ptr(), logits.data_ptr(),
+                                (const int32_t *)row_start.data_ptr(), most ? (const int64_t *)drafts.data_ptr() : nullptr,
+                                most ? (const float *)accept_uniforms.data_ptr() : nullptr,
+                                (const float *)sample_uniforms.data_ptr(), (const float *)optional_ptr(temperatures), batch,
+                                max_drafts, logits.size(0), vocab, logits.stride(0), drafts.stride(0),
+                                accept_uniforms.stride(0), code, workspace.data_ptr(), bytes, device.stream()));
+  return std::make_tuple(tokens, counts);
 }
 
 }  // namespace arctic_host

@@ -88,4 +88,16 @@ void move_rows(const char *fn, const TensorList &sources, const at::Tensor &indi
 // torch.argmax(logits, -1).clamp_(0, max_index) (arctic_speculator.py:846-848, 862)
 at::Tensor argmax_clamp(const at::Tensor &logits, int64_t max_index);
 
+// Attention of new tokens over one layer's paged caches into `out`: [batch(, new tokens), heads, head_size], or with
+// query_start ragged runs of them, [tokens, heads, head_size].  window 0: no limit.
+void paged_attention(const at::Tensor &query, const OptTensor &query_start, const at::Tensor &key_cache,
+                     const at::Tensor &value_cache, const at::Tensor &block_table, const at::Tensor &seq_lens,
+                     const std::string &kv_cache_dtype, const at::Tensor &k_scale, const at::Tensor &v_scale, double scale,
+                     int64_t max_seq_len, int64_t window, int64_t num_sinks, const at::Tensor &out);
+
+// Verification of drafted tokens: (accepted drafts and the token behind them, how many tokens that is).
+std::tuple<at::Tensor, at::Tensor> verify_drafts(const at::Tensor &logits, const at::Tensor &row_start,
+                                                 const at::Tensor &drafts, const at::Tensor &accept_uniforms,
+                                                 const at::Tensor &sample_uniforms, const OptTensor &temperatures);
+
 }  // namespace arctic_host

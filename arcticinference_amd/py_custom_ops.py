@@ -70,6 +70,17 @@ _EXTRA_SCHEMAS = {
         "Tensor(d!)[] value_caches, Tensor slot_mapping, str kv_cache_dtype, Tensor(e)[] k_scales, "
         "Tensor(f)[] v_scales, int num_heads, int head_size, Tensor logits_indices, Tensor(g!) k_out, "
         "Tensor(h!) v_out) -> ()",
+    "paged_attention":
+        "paged_attention(Tensor query, Tensor key_cache, Tensor value_cache, Tensor block_table, Tensor seq_lens, "
+        "str kv_cache_dtype, Tensor k_scale, Tensor v_scale, float scale, int max_seq_len, int window, int num_sinks, "
+        "Tensor(a!) out) -> ()",
+    "paged_attention_ragged":
+        "paged_attention_ragged(Tensor query, Tensor query_start, Tensor key_cache, Tensor value_cache, "
+        "Tensor block_table, Tensor seq_lens, str kv_cache_dtype, Tensor k_scale, Tensor v_scale, float scale, "
+        "int max_seq_len, int window, int num_sinks, Tensor(a!) out) -> ()",
+    "verify_draft_tokens":
+        "verify_draft_tokens(Tensor logits, Tensor row_start, Tensor draft_token_ids, Tensor accept_uniforms, "
+        "Tensor sample_uniforms, Tensor? temperatures) -> (Tensor, Tensor)",
     "gather_rows": "gather_rows(Tensor[] sources, Tensor indices, Tensor(a!)[] outs) -> ()",
     "scatter_rows": "scatter_rows(Tensor[] sources, Tensor indices, Tensor(a!)[] outs) -> ()",
 }
@@ -123,6 +134,12 @@ def _meta_argmax(logits, max_index):
     return torch.empty(logits.shape[:-1], dtype=torch.int64, device=logits.device)
 
 
+def _meta_verify(logits, row_start, draft_token_ids, *args):
+    batch, drafts = draft_token_ids.shape
+    return (torch.empty((batch, drafts + 1), dtype=torch.int64, device=logits.device),
+            torch.empty((batch,), dtype=torch.int64, device=logits.device))
+
+
 def _meta_nothing(*args):
     return None
 
@@ -139,6 +156,9 @@ _META_IMPLS = {
     "reshape_and_cache_flash_bulk": _meta_nothing,
     "reshape_and_cache_flash_bulk_select": _meta_nothing,
     "reshape_and_cache_flash_fp4": _meta_nothing,
+    "paged_attention": _meta_nothing,
+    "paged_attention_ragged": _meta_nothing,
+    "verify_draft_tokens": _meta_verify,
     "gather_rows": _meta_nothing,
     "scatter_rows": _meta_nothing,
 }
@@ -439,3 +459,99 @@ def speculator_argmax(logits: torch.Tensor, vocab_size: int) -> torch.Tensor:
     selection at the end of a speculator step (arctic_inference/vllm/spec_dec/arctic_speculator.py:846-848,
     862).  Same winner as torch: lowest index among equal values, a NaN beats every number."""
     return _call("speculator_argmax_cuda", logits, int(vocab_size) - 1)
+
+
+def paged_attention(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    kv_cache_dtype: str,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    scale: float,
+    max_seq_len: int,
+    window: Optional[int] = None,
+    num_sinks: int = 0,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """Attention of each sequence's newest tokens over one layer's paged caches, as the bulk write fills them.
+
+    ``query`` is ``[batch, heads, head_size]`` (one new token each) or ``[batch, new_tokens, heads, head_size]`` (drafted
+    tokens that are verified together); the last ``new_tokens`` of the ``seq_lens[b]`` tokens (int32) that sequence b has
+    in the cache are its queries, each sees the tokens up to itself.  With ``window`` it sees the last ``window`` of them
+    and the first ``num_sinks``.  ``key_cache`` / ``value_cache`` are ``[blocks, block_size, kv_heads, head_size]`` of the
+    queries' type (``"auto"``) or of fp8 bytes (``"fp8"``, ``"fp8_e4m3"``, ``"fp8_e5m2"``, times ``k_scale`` /
+    ``v_scale``, one fp32 each); ``heads`` is a multiple of ``kv_heads``.  ``block_table`` is int32
+    ``[batch, blocks]``; an entry outside the cache holds no keys.  ``max_seq_len``, the longest of ``seq_lens`` or more,
+    is what the work is split by; results do not depend on it beyond their rounding.  A query that sees nothing (a
+    sequence shorter than its queries) answers zeros.  Returns ``out``, which is made if it is not given.  Not in the
+    reference, whose layers leave attention to the serving engine
+    (arctic_inference/vllm/swiftkv/llama_swiftkv.py:617-622 is the write in front of it)."""
+    if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    _call("paged_attention", query, key_cache, value_cache, block_table, seq_lens, kv_cache_dtype, k_scale, v_scale,
+          scale, max_seq_len, _window(window), num_sinks, out)
+    return out
+
+
+def paged_attention_ragged(
+    query: torch.Tensor,
+    query_start: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    kv_cache_dtype: str,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+    scale: float,
+    max_seq_len: int,
+    window: Optional[int] = None,
+    num_sinks: int = 0,
+    out: Optional[torch.Tensor] = None,
+) -> torch.Tensor:
+    """``paged_attention`` for runs of new tokens of any length (prompts, chunks of prompts, decode tokens among them):
+    ``query`` is ``[tokens, heads, head_size]``, rows ``query_start[b]`` to ``query_start[b + 1] - 1`` (int32,
+    ``batch + 1`` entries) are the last tokens of sequence b.  Rows behind the last sequence are left as they were."""
+    if out is None:
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+    _call("paged_attention_ragged", query, query_start, key_cache, value_cache, block_table, seq_lens, kv_cache_dtype,
+          k_scale, v_scale, scale, max_seq_len, _window(window), num_sinks, out)
+    return out
+
+
+def _window(window: Optional[int]) -> int:
+    if window is None:
+        return 0
+    if window < 1:
+        raise ValueError(f"window must be at least 1, or None for no limit; got {window}")
+    return window
+
+
+def verify_draft_tokens(
+    target_logits: torch.Tensor,
+    row_start: torch.Tensor,
+    draft_token_ids: torch.Tensor,
+    accept_uniforms: torch.Tensor,
+    sample_uniforms: torch.Tensor,
+    temperatures: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Which drafted tokens the target model accepts, and the token behind them, from given random numbers.
+
+    Request b has ``n = row_start[b + 1] - row_start[b] - 1`` drafts, the first n of row b of ``draft_token_ids`` (int64
+    ``[batch, drafts]``), and n + 1 rows of ``target_logits`` (``[rows, vocab_size]``, fp32, fp16 or bf16): those at its
+    drafts' places and the one behind.  With a row's probabilities p (softmax of the logits over ``temperatures[b]``,
+    1 without them) draft d is accepted iff ``accept_uniforms[b, k] < p[d]``; the token behind the accepted ones is drawn
+    by inversion of ``sample_uniforms[b]`` from the first row that was not accepted, without its draft, or from the last
+    row: the distribution is the target's whatever was drafted, as long as every draft is one token and no sample of a
+    distribution (the argmax speculators' and the suffix tree's are).  A temperature that is not positive stands for the
+    argmax: accepted iff equal to it.  A row without a distribution (all -inf, a +inf, a NaN, or no weight but the
+    rejected draft's) answers its argmax.  Returns ``(tokens, counts)``: int64 ``[batch, drafts + 1]``, the accepted
+    drafts, the token behind them, -1; and int64 ``[batch]``, how many tokens that is (0 for a request without rows).
+    Uniform numbers are in [0, 1).  The drafts are the speculator's
+    (arctic_inference/vllm/spec_dec/arctic_speculator.py:846-862); the reference leaves this step to the serving
+    engine's rejection sampler."""
+    return _call("verify_draft_tokens", target_logits, row_start, draft_token_ids, accept_uniforms, sample_uniforms,
+                 temperatures)

@@ -419,6 +419,116 @@ int arctic_argmax_clamp_split(int64_t *out, const void *logits, int64_t rows, in
                               int64_t row_stride, int64_t max_index, int dtype, void *workspace,
                               int64_t workspace_bytes, void *stream);
 
+/*
+ * A paged key-value cache of one layer, as arctic_reshape_and_cache_flash_bulk writes it: token `slot` of a sequence
+ * lies in block slot / block_size at offset slot % block_size.
+ *
+ *   key_cache, value_cache   device; element (block, offset, head, i) is block * *_block_stride + offset *
+ *                 *_token_stride + head * *_head_stride + i ELEMENTS from the start (heads behind tokens or before them)
+ *   k_scale, v_scale   device, one fp32 each, read when the kernel runs: what an element of an fp8 cache is multiplied
+ *                 by.  Ignored for ARCTIC_KV_AUTO, whose elements are of the queries' type.
+ */
+typedef struct arctic_paged_cache {
+  const void *key_cache;
+  const void *value_cache;
+  const float *k_scale;
+  const float *v_scale;
+  int64_t num_blocks;
+  int64_t key_block_stride, key_token_stride, key_head_stride;
+  int64_t value_block_stride, value_token_stride, value_head_stride;
+  int block_size;
+  int num_kv_heads;
+  int head_size;
+  int kv_cache_dtype;
+} arctic_paged_cache;
+
+/*
+ * Attention of the newest tokens of each sequence over the paged cache: of the one token of a decode step, or of the
+ * few drafted ones that are verified together.  The reference leaves attention to its serving engine's backends; its
+ * layers call them behind the cache write (arctic_inference/vllm/swiftkv/llama_swiftkv.py:617-622).
+ *
+ * Sequence b has seq_lens[b] tokens in the cache, its new ones among them; the last new_tokens of them are its queries:
+ * query i is at position p = seq_lens[b] - new_tokens + i.  It sees the keys j <= p with j > p - window (window > 0) or
+ * j < num_sinks, and head h reads key head h / (num_heads / num_kv_heads):
+ *   s_j = scale * k_scale * <query, K_j>;  out = v_scale * sum_j exp(s_j - max s) V_j / sum_j exp(s_j - max s)
+ * with sums, scores and statistics in fp32, rounded once into the queries' type.  (For fp16 and bf16 queries the weights
+ * exp(s_j - max s) are rounded to that type before they multiply V; their sum takes them rounded as well.)  A query that
+ * sees no key (p < 0) answers zeros.  What lies at keys that a query does not see does not matter, NaN and infinities
+ * among it.
+ *
+ *   query       device; [batch * new_tokens][num_heads][head_size], strides in ELEMENTS, innermost dense
+ *   out         device, likewise
+ *   block_table device int32 [batch][max_blocks], rows table_stride entries apart: the blocks of sequence b in order.
+ *               An entry outside [0, num_blocks) holds no keys.
+ *   seq_lens    device int32 [batch]; a length beyond max_blocks * block_size counts as that, a negative one as 0
+ *   max_seq_len what the work is split by: the longest of seq_lens, or more.  Results are right whatever it says.
+ *   window      0: no limit.  num_sinks matters with a window only.
+ *   head_size   at most 512
+ *   workspace   device, 16-byte aligned, at least arctic_paged_attention_workspace_bytes(...) of the same arguments (0:
+ *               may be NULL); of this call alone until its kernels have run, contents do not matter
+ */
+int64_t arctic_paged_attention_workspace_bytes(int64_t batch, int new_tokens, int num_heads,
+                                               const arctic_paged_cache *cache, int64_t max_seq_len, int64_t window,
+                                               int64_t num_sinks, int dtype);
+int arctic_paged_attention(void *out, const void *query, const arctic_paged_cache *cache,
+                           const int32_t *block_table, const int32_t *seq_lens, int64_t batch, int new_tokens,
+                           int num_heads, int64_t max_blocks, int64_t table_stride, int64_t query_token_stride,
+                           int64_t query_head_stride, int64_t out_token_stride, int64_t out_head_stride, float scale,
+                           int64_t max_seq_len, int64_t window, int64_t num_sinks, int dtype, void *workspace,
+                           int64_t workspace_bytes, void *stream);
+
+/*
+ * The same for runs of new tokens of any length: whole prompts, chunks of prompts, decode tokens among them.
+ *
+ *   query_start device int32 [batch + 1], not decreasing: the queries of sequence b are rows query_start[b] to
+ *               query_start[b + 1] - 1, and its last tokens.  Rows behind the last sequence are left as they were.
+ *   total_tokens   rows of query and out
+ */
+int64_t arctic_paged_attention_ragged_workspace_bytes(int64_t batch, int64_t total_tokens, int num_heads,
+                                                      const arctic_paged_cache *cache, int64_t max_seq_len,
+                                                      int64_t window, int64_t num_sinks, int dtype);
+int arctic_paged_attention_ragged(void *out, const void *query, const int32_t *query_start,
+                                  const arctic_paged_cache *cache, const int32_t *block_table, const int32_t *seq_lens,
+                                  int64_t batch, int64_t total_tokens, int num_heads, int64_t max_blocks,
+                                  int64_t table_stride, int64_t query_token_stride, int64_t query_head_stride,
+                                  int64_t out_token_stride, int64_t out_head_stride, float scale, int64_t max_seq_len,
+                                  int64_t window, int64_t num_sinks, int dtype, void *workspace,
+                                  int64_t workspace_bytes, void *stream);
+
+/*
+ * Verification of drafted tokens against the target model's logits, from given random numbers.  The reference leaves it
+ * to its serving engine's rejection sampler; the drafts are those of its speculators and of its suffix tree
+ * (arctic_inference/vllm/spec_dec/arctic_speculator.py:846-862), which propose one token at each place and no
+ * distribution.
+ *
+ * Request b has n = row_start[b + 1] - row_start[b] - 1 drafts (0 to max_drafts) and the n + 1 rows of logits x that the
+ * target gave for the places of its drafts and for the place behind the last one.  With w_j = exp((x_j - max x) / T):
+ *   draft d of row k is accepted iff accept_uniforms[b][k] * sum_j w_j < w_d;  a = the accepted drafts before the first
+ *   that is not;  the token behind them is the smallest j with sum_{i <= j} w_i > sample_uniforms[b] * sum_i w_i over
+ *   row a, from whose weights a rejected draft is left out
+ * which leaves the target's own distribution, whatever was drafted.  T = temperatures[b]; where that is not positive a
+ * draft is accepted iff it is the row's argmax (lowest index among equal values) and the token behind is the argmax.
+ * A row without a distribution (nothing but -inf, a +inf, a NaN) accepts no draft and answers its argmax (the first
+ * NaN), and so does one that has no weight but its rejected draft's; a draft outside [0, vocab_size) is never accepted.  Sums and their weights are held in 64 bits, since what they
+ * are compared with decides a whole number.
+ *
+ *   out_tokens   device int64 [batch][max_drafts + 1]: the accepted drafts, the token behind them, -1
+ *   out_counts   device int64 [batch]: a + 1; 0 for a request without rows
+ *   logits       device; num_rows rows of vocab_size elements (F32, F16 or BF16), row_stride ELEMENTS apart
+ *   row_start    device int32 [batch + 1]; rows outside [0, num_rows) are not there
+ *   drafts       device int64 [batch][max_drafts], rows draft_stride apart (NULL for max_drafts == 0)
+ *   accept_uniforms   device fp32 [batch][max_drafts], rows accept_stride apart (likewise);  sample_uniforms [batch]
+ *   temperatures device fp32 [batch]; NULL: 1 for every request
+ *   workspace    device, 8-byte aligned, at least arctic_verify_drafts_workspace_bytes(...) bytes, of this call alone
+ *                until its kernels have run; contents do not matter
+ */
+int64_t arctic_verify_drafts_workspace_bytes(int64_t batch, int max_drafts, int vocab_size, int dtype);
+int arctic_verify_drafts(int64_t *out_tokens, int64_t *out_counts, const void *logits, const int32_t *row_start,
+                         const int64_t *drafts, const float *accept_uniforms, const float *sample_uniforms,
+                         const float *temperatures, int64_t batch, int max_drafts, int64_t num_rows, int vocab_size,
+                         int64_t row_stride, int64_t draft_stride, int64_t accept_stride, int dtype, void *workspace,
+                         int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
