@@ -252,8 +252,8 @@ static bool few_takes(const AttentionParams &p) {
   return wide % 16 == 0 && p.key_token < (1 << 26) && p.value_token < (1 << 26) && p.num_blocks > 0 && p.max_blocks > 0;
 }
 
-static int64_t few_bytes(const FewShape &f, int64_t new_tokens, int num_heads, int head_size) {
-  return f.least == 0 ? 0 : new_tokens * num_heads * 2 * f.workers * ((int64_t)head_size + 2) * 4;
+static int64_t few_bytes(const FewShape &f, int64_t batch, int64_t new_tokens, int num_heads, int head_size) {
+  return f.least == 0 ? 0 : new_tokens * num_heads * 2 * f.workers * ((int64_t)head_size + 2) * 4 + batch * (int64_t)sizeof(int2);
 }
 
 extern "C" int64_t arctic_paged_attention_workspace_bytes(int64_t batch, int new_tokens, int num_heads,
@@ -266,7 +266,7 @@ extern "C" int64_t arctic_paged_attention_workspace_bytes(int64_t batch, int new
     return 0;
   FewShape f;
   return few_shape(f, batch, new_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype)
-             ? few_bytes(f, new_tokens, num_heads, cache->head_size)
+             ? few_bytes(f, batch, new_tokens, num_heads, cache->head_size)
              : 0;
 }
 
@@ -289,7 +289,7 @@ extern "C" int arctic_paged_attention(void *out, const void *query, const arctic
   p.by_new = Divisor((uint32_t)new_tokens);
   FewShape f;
   if (few_takes(p) && few_shape(f, batch, new_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype)) {
-    const int64_t need = few_bytes(f, new_tokens, num_heads, cache->head_size);
+    const int64_t need = few_bytes(f, batch, new_tokens, num_heads, cache->head_size);
     if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
       return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned and hold %lld bytes", fn, (long long)need);
     FewParams fp;
@@ -301,7 +301,9 @@ extern "C" int arctic_paged_attention(void *out, const void *query, const arctic
     fp.by_row_tiles = Divisor((uint32_t)f.row_tiles);
     fp.by_head_groups = Divisor((uint32_t)(p.kv_heads / f.heads));
     fp.partial = (float *)workspace;
-    fp.statistics = need ? fp.partial + (int64_t)new_tokens * num_heads * 2 * f.workers * p.head_size : nullptr;
+    const int64_t pieces = (int64_t)new_tokens * num_heads * 2 * f.workers;
+    fp.statistics = need ? fp.partial + pieces * p.head_size : nullptr;
+    fp.dealt = need ? (int2 *)(fp.statistics + pieces * 2) : nullptr;
     if (dtype == ARCTIC_DTYPE_BF16) few_launch_bf16(fp, f, cache->kv_cache_dtype, (hipStream_t)stream);
     else few_launch_f16(fp, f, cache->kv_cache_dtype, (hipStream_t)stream);
     return check_launch(fn);

@@ -114,6 +114,7 @@ struct FewParams {
   AttentionParams a;
   float *partial;        // [kv_heads][2 * workers][rows][head_size]
   float *statistics;     // [kv_heads][2 * workers][rows][2]: maximum (base 2), sum
+  int2 *dealt;           // [batch]: the first and the last worker that a sequence was dealt to
   int rows;              // new_tokens * group
   int row_tiles;         // workgroups that share the rows
   int workers;           // workgroups that share the keys of one head (and of one row tile)
@@ -133,57 +134,68 @@ struct Tiles {
   }
   __device__ __forceinline__ int start(int t) const { return (t < sink_tiles ? t : window_tile + (t - sink_tiles)) << 5; }
 };
-// Where the sequences' tiles begin in the row of all of them, by one wave.
+// How the sequences' tiles, one sequence behind the other, are dealt out: found by every wave for itself.
 struct Deal {
-  int64_t total;   // tiles of all sequences
-  int64_t per;     // of a worker
-  __device__ __forceinline__ static int count(const AttentionParams &p, int b) {
-    return b < p.batch ? Tiles(p, clamped_length(p, b), p.new_tokens).count : 0;
-  }
-  __device__ __forceinline__ Deal(const FewParams &fp, int lane) {
-    int64_t mine = 0;
-    for (int b = lane; b < fp.a.batch; b += 64) mine += count(fp.a, b);
-    total = wave_sum_of(mine);
-    per = max((int64_t)fp.least, (total + fp.workers - 1) / fp.workers);
-  }
-  __device__ __forceinline__ static int64_t wave_sum_of(int64_t v) {
+  int64_t at, stop;   // a worker's tiles
+  int64_t begin;      // the first tile of sequence b, which tile `at` belongs to
+  int64_t per;        // tiles of a worker
+  int b;
+  __device__ __forceinline__ static int64_t up_to(int64_t v, int lane) {
 #pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t other = __shfl_up(v, d);
+      if (lane >= d) v += other;
+    }
     return v;
   }
-  // the sequence that tile `at` (of all) belongs to, and the sequence's first tile
-  __device__ __forceinline__ static int sequence_at(const AttentionParams &p, int64_t at, int lane, int64_t *begin) {
+  __device__ __forceinline__ Deal(const FewParams &fp, int worker) {
+    const AttentionParams &p = fp.a;
+    const int lane = threadIdx.x & 63;
+    auto count = [&](int i) { return i < p.batch ? Tiles(p, clamped_length(p, i), p.new_tokens).count : 0; };
+    const int n = count(lane);
+    const int64_t upto = up_to(n, lane);
+    int64_t total = __shfl(upto, 63);
+    if (p.batch > 64) {
+      int64_t rest = 0;
+      for (int i = 64 + lane; i < p.batch; i += 64) rest += count(i);
+      total += __shfl(up_to(rest, lane), 63);
+    }
+    per = max((int64_t)fp.least, (total + fp.workers - 1) / fp.workers);
+    at = (int64_t)worker * per;
+    stop = min(total, at + per);
+    b = 0;
+    begin = 0;
+    if (at >= stop) return;
     int64_t before = 0;
-    for (int b0 = 0;; b0 += 64) {
-      const int n = count(p, b0 + lane);
-      int64_t upto = n;
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) {
-        const int64_t other = __shfl_up(upto, d);
-        if (lane >= d) upto += other;
+    for (int b0 = 0; b0 < p.batch; b0 += 64) {
+      const int own = b0 ? count(b0 + lane) : n;
+      const int64_t now = before + (b0 ? up_to(own, lane) : upto);
+      const uint64_t beyond = __ballot(now > at);
+      if (beyond) {
+        const int l = __builtin_ctzll(beyond);
+        begin = __shfl(now - own, l);
+        b = b0 + l;
+        return;
       }
-      upto += before;
-      const uint64_t beyond = __ballot(upto > at);
-      if (beyond || b0 + 64 >= p.batch) {
-        const int l = beyond ? __builtin_ctzll(beyond) : 63;
-        *begin = __shfl(upto - n, l);
-        return min(b0 + l, p.batch - 1);
-      }
-      before = __shfl(upto, 63);
+      before = __shfl(now, 63);
     }
   }
 };
 
 constexpr int kFewWaves = 4;
 
-// Waves on a SIMD, which is what a kernel's registers are allotted by: as many as hold the tiles without spilling.
-constexpr int few_waves(int padded, int columns) { return padded * columns <= 64 ? 4 : padded * columns <= 128 ? 3 : padded * columns <= 256 ? 2 : 1; }
+// Waves on a SIMD, which is what a kernel's registers are allotted by: K and V of a tile, the query rows, their results
+// and about 70 more have to fit without spilling.  (Two, a workgroup's waves over, already read at the full rate.)
+constexpr int few_waves(int padded, int element, int columns) {
+  const int registers = padded * element / 4 + columns * (padded * 3 / 8 + 8) + 70;
+  return registers <= 168 ? 3 : registers <= 256 ? 2 : 1;
+}
 
 // kPadded: head size that the products are made for; kColumns: column tiles of 16 query rows; kHeads: key heads that a
 // workgroup's waves share (rows of 128 bytes or less lie side by side in one stretch of memory); kPlain: the head fills
 // kPadded and 16 keys that start at a multiple of 16 lie in one block.
 template <typename T, typename C, int kPadded, int kColumns, int kHeads, bool kPlain>
-__global__ __launch_bounds__(64 * kFewWaves, few_waves(kPadded, kColumns)) void attention_few_kernel(const FewParams fp) {
+__global__ __launch_bounds__(64 * kFewWaves, few_waves(kPadded, C::kBytes, kColumns)) void attention_few_kernel(const FewParams fp) {
   const AttentionParams &p = fp.a;
   constexpr int kElt = C::kBytes;
   constexpr int kSteps = kPadded / 32;             // of the first product
@@ -206,14 +218,12 @@ __global__ __launch_bounds__(64 * kFewWaves, few_waves(kPadded, kColumns)) void 
   const u32x4 ones = {one, one, one, one};
 
   int b = worker;
-  int64_t at = 0, stop = 0, begin = 0;   // of the row of all tiles: what is left to do, and where sequence b begins
+  int64_t at = 0, stop = 0, begin = 0, per = 1;   // of the row of all tiles: what is left to do, and where sequence b begins
   if (fp.least) {
-    const int lane = threadIdx.x & 63;
-    const Deal deal(fp, lane);
-    at = (int64_t)worker * deal.per;
-    stop = min(deal.total, at + deal.per);
+    const Deal deal(fp, worker);
+    at = deal.at, stop = deal.stop, begin = deal.begin, per = deal.per;
     if (at >= stop) return;
-    b = __builtin_amdgcn_readfirstlane(Deal::sequence_at(p, at, lane, &begin));
+    b = __builtin_amdgcn_readfirstlane(deal.b);
   }
   for (;;) {
   // (the lane's number as if it were another for every piece: what follows from it is then computed where it is needed and
@@ -548,6 +558,8 @@ __global__ __launch_bounds__(64 * kFewWaves, few_waves(kPadded, kColumns)) void 
     }
     __syncthreads();
   }
+  if (fp.least && first == 0 && kv_head == 0 && row0 == 0 && wave == 0 && lane == 0)
+    fp.dealt[b] = make_int2((int)(begin / per), (int)((begin + tiles.count - 1) / per));
   // a head's result by its waves; a worker has at most one piece that goes on with a sequence (the first place) and one
   // that begins one and does not end it (the second)
   const int64_t place = (int64_t)kv_head * 2 * fp.workers + 2 * worker + (first == 0 ? 1 : 0);
@@ -597,39 +609,68 @@ __global__ __launch_bounds__(64 * kFewWaves, few_waves(kPadded, kColumns)) void 
 }
 
 // Sequences that were dealt to several workers: out = v_scale sum_w 2^(m_w - M) o_w / sum_w 2^(m_w - M) l_w, a wave per
-// row.
-template <typename T>
-__global__ __launch_bounds__(64) void attention_join_kernel(const FewParams fp) {
+// row.  kPadded / 4 lanes take a piece's values, 256 / kPadded pieces at a time and four such groups requested ahead.
+constexpr int kJoinWaves = 4;
+template <typename T, int kPadded>
+__global__ __launch_bounds__(64 * kJoinWaves) void attention_join_kernel(const FewParams fp) {
   const AttentionParams &p = fp.a;
-  const int lane = threadIdx.x;
-  const uint32_t token = p.by_heads.quotient(blockIdx.x);   // b * new_tokens + i
-  const int head = (int)(blockIdx.x - token * (uint32_t)p.heads);
+  constexpr int kLanes = kPadded / 4, kSide = 64 / kLanes, kAhead = 4;
+  const int lane = threadIdx.x & 63, side = lane / kLanes, d = lane % kLanes * 4;
+  const uint32_t at = blockIdx.x * kJoinWaves + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const uint32_t token = p.by_heads.quotient(at);   // b * new_tokens + i
+  if (token >= p.total_tokens) return;
+  const int head = (int)(at - token * (uint32_t)p.heads);
   const int b = (int)p.by_new.quotient(token), i = (int)token - b * p.new_tokens;
-  const Deal deal(fp, lane);
-  int64_t before = 0;
-  for (int k = lane; k < b; k += 64) before += Deal::count(p, k);
-  before = Deal::wave_sum_of(before);
-  const int64_t first = before / deal.per, last = (before + Deal::count(p, b) - 1) / deal.per;
+  const int2 dealt = fp.dealt[b];
+  const int first = dealt.x, last = dealt.y;
   if (first == last) return;   // written by the worker
   const int kv_head = (int)p.by_group.quotient((uint32_t)head);
   const int row = i * p.group + head - kv_head * p.group;
   const int64_t place = (int64_t)kv_head * 2 * fp.workers;
   // the first worker's piece begins the sequence, the others' go on with it
-  auto piece = [&](int64_t w) { return (place + 2 * w + (w == first ? 1 : 0)) * fp.rows + row; };
-  float top = -__builtin_inff();
-  for (int64_t w = first + lane; w <= last; w += 64) top = fmaxf(top, fp.statistics[piece(w) * 2]);
-  top = wave_max(top);
-  const float base = top == -__builtin_inff() ? 0.f : top;
-  float sum = 0.f;
+  auto piece = [&](int w) { return (place + 2 * w + (w == first ? 1 : 0)) * fp.rows + row; };
+  float top = -__builtin_inff(), sum = 0.f;
   f32x4 acc = {0, 0, 0, 0};
-  const int d = lane * 4;   // head sizes up to 256 come here
-  for (int64_t w = first; w <= last; ++w) {
-    const float *st = fp.statistics + piece(w) * 2;
-    const float keep = __builtin_amdgcn_exp2f(st[0] - base);
-    sum += st[1] * keep;
-    if (d < p.head_size) acc += *(const ARCTIC_GLOBAL f32x4 *)(fp.partial + piece(w) * p.head_size + d) * keep;
+  for (int w0 = first; w0 <= last; w0 += kSide * kAhead) {
+    float2 st[kAhead];
+    f32x4 part[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int w = w0 + k * kSide + side;
+      st[k] = make_float2(-__builtin_inff(), 0.f);
+      part[k] = f32x4{0, 0, 0, 0};
+      if (w <= last) {
+        st[k] = *(const float2 *)(fp.statistics + piece(w) * 2);
+        if (d < p.head_size) part[k] = *(const ARCTIC_GLOBAL f32x4 *)(fp.partial + piece(w) * p.head_size + d);
+      }
+    }
+    float now = top;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) now = fmaxf(now, st[k].x);
+    const float base = now == -__builtin_inff() ? 0.f : now, keep = __builtin_amdgcn_exp2f(top - base);
+    sum *= keep;
+    acc *= keep;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const float own = __builtin_amdgcn_exp2f(st[k].x - base);
+      sum += st[k].y * own;
+      acc += part[k] * own;
+    }
+    top = now;
   }
-  if (d >= p.head_size) return;
+  // the sides' results
+#pragma unroll
+  for (int s = kLanes; s < 64; s <<= 1) {
+    const float other = __shfl_xor(top, s), now = fmaxf(top, other), base = now == -__builtin_inff() ? 0.f : now;
+    const float keep = __builtin_amdgcn_exp2f(top - base);
+    sum *= keep;
+    acc *= keep;
+    sum += __shfl_xor(sum, s);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc[k] += __shfl_xor(acc[k], s);
+    top = now;
+  }
+  if (side || d >= p.head_size) return;
   acc *= sum == 0.f ? 0.f : (p.v_scale ? *p.v_scale : 1.f) / sum;
   *(ARCTIC_GLOBAL u32x2 *)(p.out + (int64_t)token * p.out_token + (int64_t)head * p.out_head + d * 2) =
       u32x2{T::pack(acc[0], acc[1]), T::pack(acc[2], acc[3])};
@@ -668,7 +709,11 @@ inline void few_launch(const FewParams &p, const FewShape &f, int kv, hipStream_
   if (kv == ARCTIC_KV_AUTO) few_launch_padded<T, Half<T>>(p, f, grid, s);
   else if (kv == ARCTIC_KV_FP8_E4M3) few_launch_padded<T, CacheE4M3>(p, f, grid, s);
   else few_launch_padded<T, CacheE5M2>(p, f, grid, s);
-  if (f.least) launch(attention_join_kernel<T>, dim3((unsigned)(p.a.total_tokens * p.a.heads)), 64, s, p);
+  if (!f.least) return;
+  const dim3 rows((unsigned)((p.a.total_tokens * p.a.heads + kJoinWaves - 1) / kJoinWaves));
+  if (f.padded == 64) launch(attention_join_kernel<T, 64>, rows, 64 * kJoinWaves, s, p);
+  else if (f.padded == 128) launch(attention_join_kernel<T, 128>, rows, 64 * kJoinWaves, s, p);
+  else launch(attention_join_kernel<T, 256>, rows, 64 * kJoinWaves, s, p);
 }
 
 }  // namespace arctic
