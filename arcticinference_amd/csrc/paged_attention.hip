@@ -11,7 +11,7 @@
 #include <algorithm>
 #include <cstdint>
 
-#include "paged_attention_few.hpp"
+#include "paged_attention_many.hpp"
 
 namespace arctic {
 
@@ -256,6 +256,59 @@ static int64_t few_bytes(const FewShape &f, int64_t batch, int64_t new_tokens, i
   return f.least == 0 ? 0 : new_tokens * num_heads * 2 * f.workers * ((int64_t)head_size + 2) * 4 + batch * (int64_t)sizeof(int2);
 }
 
+// ---- many ------------------------------------------------------------------------------------------------------
+
+// `total_tokens` query tokens of `batch` sequences, new_tokens of each or (0) ragged.
+static bool many_shape(ManyShape &f, int64_t batch, int64_t new_tokens, int64_t total_tokens, int num_heads,
+                       const arctic_paged_cache &c, int64_t max_seq_len, int64_t window, int64_t num_sinks, int dtype) {
+  if (dtype == ARCTIC_DTYPE_F32 || c.head_size > 256 || c.head_size % (c.kv_cache_dtype == ARCTIC_KV_AUTO ? 8 : 16)) return false;
+  const int64_t group = num_heads / c.num_kv_heads, rows = total_tokens * group;
+  f.padded = c.head_size <= 64 ? 64 : c.head_size <= 128 ? 128 : 256;
+  f.waves = f.padded == 256 || rows * c.num_kv_heads < 256 * 256 ? 4 : 8;
+  const int64_t tile = 32 * f.waves;
+  f.per_sequence = (int)std::min<int64_t>((new_tokens * group + tile - 1) / tile, 0x7fffffff);
+  f.slots = new_tokens ? batch * f.per_sequence : rows / tile + batch;
+  // The row tiles that there are for sure: rows / tile; splits where they leave CUs idle.
+  const int64_t units = std::max<int64_t>(1, rows / tile) * c.num_kv_heads;
+  const int64_t tiles = (most_tiles(max_seq_len, tile / group + 1, window, num_sinks) + 1) / 2;
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(256 / units, (tiles + 7) / 8));
+  f.tiles_per_split = (int)((tiles + splits - 1) / splits);
+  f.splits = (int)((tiles + f.tiles_per_split - 1) / f.tiles_per_split);
+  return f.slots * f.splits * c.num_kv_heads <= 0x7fffffffLL;
+}
+
+static int64_t many_bytes(const ManyShape &f, int num_kv_heads, int head_size) {
+  return f.splits == 1 ? 0 : f.slots * num_kv_heads * f.splits * 32 * f.waves * ((int64_t)head_size + 2) * 4;
+}
+
+static int workspace_error(const char *fn, int64_t need) {
+  return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned and hold %lld bytes", fn, (long long)need);
+}
+
+static int run_many(const char *fn, const AttentionParams &p, const ManyShape &f, int dtype, int kv, void *workspace,
+                    int64_t workspace_bytes, hipStream_t s) {
+  const int64_t need = many_bytes(f, p.kv_heads, p.head_size);
+  if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)) return workspace_error(fn, need);
+  ManyParams mp;
+  mp.a = p;
+  mp.slots = (int)f.slots;
+  mp.splits = f.splits;
+  mp.tiles_per_split = f.tiles_per_split;
+  mp.per_sequence = f.per_sequence;
+  mp.by_kv_heads = Divisor((uint32_t)p.kv_heads);
+  mp.by_splits = Divisor((uint32_t)f.splits);
+  mp.by_per_sequence = Divisor((uint32_t)std::max(1, f.per_sequence));
+  mp.by_group = Divisor((uint32_t)p.group);
+  mp.partial = need ? (float *)workspace : nullptr;
+  mp.statistics = need ? mp.partial + f.slots * p.kv_heads * f.splits * 32 * f.waves * p.head_size : nullptr;
+  if (dtype == ARCTIC_DTYPE_BF16) many_launch_bf16(mp, f, kv, s);
+  else many_launch_f16(mp, f, kv, s);
+  return check_launch(fn);
+}
+
+// Query rows of a key head beyond which the kernel for many tokens is the faster one.
+constexpr int64_t kMostFewRows = 64;
+
 extern "C" int64_t arctic_paged_attention_workspace_bytes(int64_t batch, int new_tokens, int num_heads,
                                                           const arctic_paged_cache *cache, int64_t max_seq_len,
                                                           int64_t window, int64_t num_sinks, int dtype) {
@@ -265,6 +318,11 @@ extern "C" int64_t arctic_paged_attention_workspace_bytes(int64_t batch, int new
       window < 0 || num_sinks < 0 || batch * new_tokens > 0x7fffffffLL / num_heads)
     return 0;
   FewShape f;
+  ManyShape m;
+  if (new_tokens * (int64_t)(num_heads / cache->num_kv_heads) > kMostFewRows)
+    return many_shape(m, batch, new_tokens, batch * new_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype)
+               ? many_bytes(m, cache->num_kv_heads, cache->head_size)
+               : 0;
   return few_shape(f, batch, new_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype)
              ? few_bytes(f, batch, new_tokens, num_heads, cache->head_size)
              : 0;
@@ -288,10 +346,13 @@ extern "C" int arctic_paged_attention(void *out, const void *query, const arctic
   p.new_tokens = new_tokens;
   p.by_new = Divisor((uint32_t)new_tokens);
   FewShape f;
-  if (few_takes(p) && few_shape(f, batch, new_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype)) {
+  ManyShape m;
+  if ((int64_t)new_tokens * p.group > kMostFewRows) {
+    if (few_takes(p) && many_shape(m, batch, new_tokens, p.total_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype))
+      return run_many(fn, p, m, dtype, cache->kv_cache_dtype, workspace, workspace_bytes, (hipStream_t)stream);
+  } else if (few_takes(p) && few_shape(f, batch, new_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype)) {
     const int64_t need = few_bytes(f, batch, new_tokens, num_heads, cache->head_size);
-    if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
-      return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: the workspace must be 16-byte aligned and hold %lld bytes", fn, (long long)need);
+    if (need && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need)) return workspace_error(fn, need);
     FewParams fp;
     fp.a = p;
     fp.rows = new_tokens * p.group;
@@ -314,8 +375,14 @@ extern "C" int arctic_paged_attention(void *out, const void *query, const arctic
 extern "C" int64_t arctic_paged_attention_ragged_workspace_bytes(int64_t batch, int64_t total_tokens, int num_heads,
                                                                  const arctic_paged_cache *cache, int64_t max_seq_len,
                                                                  int64_t window, int64_t num_sinks, int dtype) {
-  (void)batch, (void)total_tokens, (void)num_heads, (void)cache, (void)max_seq_len, (void)window, (void)num_sinks, (void)dtype;
-  return 0;
+  if (!cache || batch <= 0 || batch > 0x7ffffffeLL || total_tokens <= 0 || num_heads <= 0 || num_heads > (1 << 20) ||
+      cache->num_kv_heads <= 0 || num_heads % cache->num_kv_heads || cache->head_size <= 0 || cache->block_size <= 0 || max_seq_len < 0 ||
+      window < 0 || num_sinks < 0 || total_tokens > 0x7fffffffLL / num_heads)
+    return 0;
+  ManyShape m;
+  return many_shape(m, batch, 0, total_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype)
+             ? many_bytes(m, cache->num_kv_heads, cache->head_size)
+             : 0;
 }
 
 extern "C" int arctic_paged_attention_ragged(void *out, const void *query, const int32_t *query_start,
@@ -333,7 +400,10 @@ extern "C" int arctic_paged_attention_ragged(void *out, const void *query, const
   if (rc != ARCTIC_OK || batch == 0 || total_tokens == 0) return rc;
   if (!query_start || (uintptr_t)query_start % 4)
     return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: query_start is missing or not aligned", fn);
-  (void)max_seq_len, (void)workspace, (void)workspace_bytes;
+  if (max_seq_len < 0) return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: max_seq_len must not be negative", fn);
   p.query_start = query_start;
+  ManyShape m;
+  if (few_takes(p) && many_shape(m, batch, 0, total_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype))
+    return run_many(fn, p, m, dtype, cache->kv_cache_dtype, workspace, workspace_bytes, (hipStream_t)stream);
   return run_attention(fn, p, dtype, cache->kv_cache_dtype, (hipStream_t)stream);
 }
