@@ -47,6 +47,34 @@ __device__ __forceinline__ float logit(const char *row, int i) {
   return kDtype == ARCTIC_DTYPE_BF16 ? BF16::lo(bits) : F16::lo(bits);
 }
 
+// kPerLane consecutive logits from `first` on, -inf for those at `end` and beyond; whole 16-byte chunks at a time, rows may
+// start anywhere.
+template <int kDtype, int kCount>
+__device__ __forceinline__ void some_logits(const char *row, int first, int end, float (&x)[kCount]) {
+  constexpr int kElt = kDtype == ARCTIC_DTYPE_F32 ? 4 : 2, kPerChunk = 16 / kElt;
+  if (first + kCount <= end) {
+    uint4 raw[kCount / kPerChunk];
+#pragma unroll
+    for (int i = 0; i < kCount / kPerChunk; ++i) raw[i] = load16<true>(row + (int64_t)(first + i * kPerChunk) * kElt);
+#pragma unroll
+    for (int i = 0; i < kCount / kPerChunk; ++i) {
+      if constexpr (kDtype == ARCTIC_DTYPE_F32) {
+        x[4 * i] = __uint_as_float(raw[i].x), x[4 * i + 1] = __uint_as_float(raw[i].y);
+        x[4 * i + 2] = __uint_as_float(raw[i].z), x[4 * i + 3] = __uint_as_float(raw[i].w);
+      } else {
+        float f[8];
+        if constexpr (kDtype == ARCTIC_DTYPE_BF16) unpack8<BF16>(raw[i], f);
+        else unpack8<F16>(raw[i], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[8 * i + j] = f[j];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) x[i] = first + i < end ? logit<kDtype>(row, first + i) : -__builtin_inff();
+  }
+}
+
 // The value that a key was made of (NaN for any NaN, -inf for no key).
 __device__ __forceinline__ float key_value(uint64_t key) {
   const uint32_t o = (uint32_t)(key >> 32);
@@ -55,16 +83,43 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   return __uint_as_float(o ^ ((o & 0x80000000u) ? 0x80000000u : 0xffffffffu));
 }
 
-// exp((x - m) / T); x = -inf has no weight whatever T says.
-__device__ __forceinline__ double weight_of(float x, float m, double inv_t) {
-  return x == -__builtin_inff() ? 0.0 : exp(((double)x - (double)m) * inv_t);
+// 2^((x - m) c) in fp64, relative error 2e-14, for (x - m) c <= 0; 0 below 2^-1074 and for x = -inf whatever c is.
+// t = n + f with n whole (found by adding 1.5 2^52, whose last bit is worth 1) and |f| <= 1/2, 2^f by its Chebyshev
+// interpolation of degree 9 there.
+__device__ __forceinline__ double weight_of(double x, double m, double c) {
+  const double t = fmax((x - m) * c, -1100.0);
+  const double shifted = t + 6755399441055744.0;
+  const int n = (int)(uint32_t)__double_as_longlong(shifted);
+  const double f = t - (shifted - 6755399441055744.0);
+  double v = 0x1.b6571ea79d565p-24;
+  v = fma(v, f, 0x1.63ef969b0e64ep-20);
+  v = fma(v, f, 0x1.ffcb7677a5f5cp-17);
+  v = fma(v, f, 0x1.43088e257e65bp-13);
+  v = fma(v, f, 0x1.5d87fe908fed1p-10);
+  v = fma(v, f, 0x1.3b2ab72b175f8p-7);
+  v = fma(v, f, 0x1.c6b08d7044115p-5);
+  v = fma(v, f, 0x1.ebfbdff8149f2p-3);
+  v = fma(v, f, 0x1.62e42fefa39f7p-1);
+  v = fma(v, f, 0x1.000000000003dp+0);
+  return __builtin_amdgcn_ldexp(v, n);
 }
+// c for temperature t: log2(e) / t
+__device__ __forceinline__ double per_unit(float t) { return 1.4426950408889634074 / (double)t; }
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
 
 __device__ __forceinline__ double wave_sum64(double v) {
 #pragma unroll
   for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+// the sum of a lane's value and those of the lanes before it
+__device__ __forceinline__ double sum_up_to(double v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const double other = __shfl_up(v, d);
+    if (lane >= d) v += other;
+  }
   return v;
 }
 
@@ -77,8 +132,9 @@ __device__ __forceinline__ int drafts_of(const VerifyParams &p, int b, int64_t *
 
 template <int kDtype>
 __global__ __launch_bounds__(kVerifyLanes) void verify_segments_kernel(const VerifyParams p) {
-  __shared__ uint64_t keys[kVerifyLanes / 64];
-  __shared__ double sums[kVerifyLanes / 64];
+  constexpr int kWaves = kVerifyLanes / 64, kChunk = kDtype == ARCTIC_DTYPE_F32 ? 4 : 8, kLoads = kVerifyPerLane / kChunk;
+  __shared__ uint64_t keys[kWaves];
+  __shared__ double sums[kWaves];
   const uint32_t place = p.by_parts.quotient(blockIdx.x);   // b * (max_drafts + 1) + k
   const int part = (int)(blockIdx.x - place * (uint32_t)p.parts);
   const int b = (int)p.by_places.quotient(place), k = (int)(place - (uint32_t)b * (uint32_t)(p.max_drafts + 1));
@@ -86,45 +142,79 @@ __global__ __launch_bounds__(kVerifyLanes) void verify_segments_kernel(const Ver
   const int n = drafts_of(p, b, &start);
   if (k > n) return;
   const char *row = p.logits + (start + k) * p.row_stride_bytes;
+  const int lane = threadIdx.x, first = part * kVerifySegment, end = min(p.vocab, first + kVerifySegment);
+  // neighbouring lanes take neighbouring chunks
+  float x[kLoads][kChunk];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) some_logits<kDtype, kChunk>(row, first + (i * kVerifyLanes + lane) * kChunk, end, x[i]);
   const float t = p.temperatures ? p.temperatures[b] : 1.f;
   const int64_t draft = k < n ? p.drafts[b * p.draft_stride + k] : -1;
-  const int lane = threadIdx.x, first = part * kVerifySegment, end = min(p.vocab, first + kVerifySegment);
-  float x[kVerifyPerLane];
-  uint64_t key = 0;
+  // the lane's maximum; a NaN is above every number, and is looked for only where a sum says that there may be one
+  float top = -__builtin_inff(), probe = 0.f;
 #pragma unroll
-  for (int i = 0; i < kVerifyPerLane; ++i) {
-    const int j = first + i * kVerifyLanes + lane;
-    x[i] = -__builtin_inff();
-    if (j < end) {
-      x[i] = logit<kDtype>(row, j);
-      key = max(key, winner_key(x[i], j));
+  for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+    for (int j = 0; j < kChunk; ++j) {
+      top = fmaxf(top, x[i][j]);
+      probe += x[i][j];
     }
+  if (probe != probe) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j)
+        if (x[i][j] != x[i][j]) top = __builtin_nanf("");
   }
-  key = wave_winner(key);
-  if ((lane & 63) == 0) keys[lane >> 6] = key;
+  // the segment's maximum, then the lowest index that has it
+  const uint32_t mine = (uint32_t)(winner_key(top, 0) >> 32), wave_top = wave_max<4>(mine);
+  if ((lane & 63) == 0) keys[lane >> 6] = wave_top;
   __syncthreads();
-  key = max(max(keys[0], keys[1]), max(keys[2], keys[3]));
-  const float m = key_value(key);
+  const uint32_t all_top = max(max((uint32_t)keys[0], (uint32_t)keys[1]), max((uint32_t)keys[2], (uint32_t)keys[3]));
+  const float m = key_value((uint64_t)all_top << 32);
+  int at = 0x7fffffff;
+  if (mine == all_top) {
+#pragma unroll
+    for (int i = kLoads - 1; i >= 0; --i)
+#pragma unroll
+      for (int j = kChunk - 1; j >= 0; --j) {
+        const int index = first + (i * kVerifyLanes + lane) * kChunk + j;
+        if (index < end && (x[i][j] == m || (m != m && x[i][j] != x[i][j]))) at = index;
+      }
+  }
+  const uint32_t lowest = ~wave_max<4>(~(uint32_t)at);
   double sum = 0.0;
   if (t > 0.f && finite(m)) {
-    const double inv_t = 1.0 / (double)t;
+    const double c = per_unit(t);
 #pragma unroll
-    for (int i = 0; i < kVerifyPerLane; ++i)
-      if (first + i * kVerifyLanes + lane != draft) sum += weight_of(x[i], m, inv_t);
+    for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+      for (int j = 0; j < kChunk; ++j) {
+        const double w = weight_of(x[i][j], m, c);
+        sum += first + (i * kVerifyLanes + lane) * kChunk + j == draft ? 0.0 : w;
+      }
   }
   sum = wave_sum64(sum);
-  if ((lane & 63) == 0) sums[lane >> 6] = sum;
   __syncthreads();
-  if (lane == 0) p.segments[blockIdx.x] = {(sums[0] + sums[1]) + (sums[2] + sums[3]), key};
+  if ((lane & 63) == 0) {
+    keys[lane >> 6] = lowest;
+    sums[lane >> 6] = sum;
+  }
+  __syncthreads();
+  if (lane == 0) {
+    const uint32_t index = min(min((uint32_t)keys[0], (uint32_t)keys[1]), min((uint32_t)keys[2], (uint32_t)keys[3]));
+    p.segments[blockIdx.x] = {(sums[0] + sums[1]) + (sums[2] + sums[3]), (uint64_t)all_top << 32 | ~index};
+  }
 }
 
 template <int kDtype>
 __global__ __launch_bounds__(kVerifyLanes) void verify_requests_kernel(const VerifyParams p) {
+  constexpr int kWaves = kVerifyLanes / 64;
   __shared__ int rejected;          // the first row whose draft is not accepted, n at the end
-  __shared__ uint64_t found;        // by the first row's wave: its key
-  __shared__ double lane_sums[kVerifyLanes];
-  __shared__ int segment_at;
+  __shared__ uint64_t row_key_at;   // of that row
   __shared__ double target_at;
+  __shared__ int segment_at;
+  __shared__ double wave_sums[kWaves];
+  __shared__ int passes_at[kWaves], some_at[kWaves];
   const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   int64_t start;
   const int n = drafts_of(p, b, &start);
@@ -135,33 +225,33 @@ __global__ __launch_bounds__(kVerifyLanes) void verify_requests_kernel(const Ver
     return;
   }
   const float t = p.temperatures ? p.temperatures[b] : 1.f;
-  const double inv_t = t > 0.f ? 1.0 / (double)t : 0.0;
+  const double c = t > 0.f ? per_unit(t) : 0.0;
   const VerifySegment *segments = p.segments + (int64_t)b * (p.max_drafts + 1) * p.parts;
   if (threadIdx.x == 0) rejected = n;
   __syncthreads();
-  auto row_key = [&](int k) {
-    uint64_t key = 0;
-    for (int s = lane; s < p.parts; s += 64) key = max(key, segments[(int64_t)k * p.parts + s].key);
-    return wave_winner(key);
-  };
   // the weights of a segment, relative to the row's maximum m
-  auto segment_sum = [&](int k, int s, float m) {
-    const VerifySegment g = segments[(int64_t)k * p.parts + s];
-    const float gm = key_value(g.key);
-    return gm == -__builtin_inff() ? 0.0 : g.sum * exp(((double)gm - (double)m) * inv_t);
+  auto segment_sum = [&](const VerifySegment &g, float m) {
+    const float own = key_value(g.key);
+    return own == -__builtin_inff() ? 0.0 : g.sum * weight_of(own, m, c);
   };
-  for (int k = wave; k < n; k += kVerifyLanes / 64) {
-    const uint64_t key = row_key(k);
-    const float m = key_value(key);
+  for (int k = wave; k < n; k += kWaves) {
     const int64_t draft = p.drafts[b * p.draft_stride + k];
+    const bool known = draft >= 0 && draft < p.vocab;
+    const float x = known ? logit<kDtype>(p.logits + (start + k) * p.row_stride_bytes, (int)draft) : 0.f;
+    const float u = p.accept[b * p.accept_stride + k];
+    const VerifySegment one = lane < p.parts ? segments[(int64_t)k * p.parts + lane] : VerifySegment{0.0, 0};
+    uint64_t key = one.key;
+    for (int s = 64 + lane; s < p.parts; s += 64) key = max(key, segments[(int64_t)k * p.parts + s].key);
+    key = wave_winner(key);
+    const float m = key_value(key);
     bool accepted = false;
-    if (finite(m) && draft >= 0 && draft < p.vocab) {
+    if (finite(m) && known) {
       if (t > 0.f) {
-        double sum = 0.0;
-        for (int s = lane; s < p.parts; s += 64) sum += segment_sum(k, s, m);
+        double sum = lane < p.parts ? segment_sum(one, m) : 0.0;
+        for (int s = 64 + lane; s < p.parts; s += 64) sum += segment_sum(segments[(int64_t)k * p.parts + s], m);
         sum = wave_sum64(sum);
-        const double own = weight_of(logit<kDtype>(p.logits + (start + k) * p.row_stride_bytes, (int)draft), m, inv_t);
-        accepted = (double)p.accept[b * p.accept_stride + k] * (sum + own) < own;
+        const double own = weight_of(x, m, c);
+        accepted = (double)u * (sum + own) < own;
       } else {
         accepted = draft == winner_index(key);
       }
@@ -172,95 +262,95 @@ __global__ __launch_bounds__(kVerifyLanes) void verify_requests_kernel(const Ver
   const int a = rejected;
   const char *row = p.logits + (start + a) * p.row_stride_bytes;
   const int64_t draft = a < n ? p.drafts[b * p.draft_stride + a] : -1;
+  for (int k = threadIdx.x; k <= p.max_drafts; k += kVerifyLanes)
+    if (k != a) tokens[k] = k < a ? p.drafts[b * p.draft_stride + k] : -1;
+  if (threadIdx.x == 0) p.out_counts[b] = a + 1;
   if (wave == 0) {
-    const uint64_t key = row_key(a);
+    const VerifySegment one = lane < p.parts ? segments[(int64_t)a * p.parts + lane] : VerifySegment{0.0, 0};
+    uint64_t key = one.key;
+    for (int s = 64 + lane; s < p.parts; s += 64) key = max(key, segments[(int64_t)a * p.parts + s].key);
+    key = wave_winner(key);
     const float m = key_value(key);
-    double total = 0.0;
-    if (t > 0.f && finite(m)) {
-      for (int s = lane; s < p.parts; s += 64) total += segment_sum(a, s, m);
-      total = wave_sum64(total);
-    }
     int at = -1;
-    double before = 0.0;
-    if (total > 0.0) {
-      // the first segment whose running sum passes the drawn number, or the last that has any weight
-      const double target = (double)p.sample[b] * total;
-      for (int s0 = 0; s0 < p.parts; s0 += 64) {
-        const double mine = s0 + lane < p.parts ? segment_sum(a, s0 + lane, m) : 0.0;
-        double upto = mine;
-        for (int d = 1; d < 64; d <<= 1) {
-          const double other = __shfl_up(upto, d);
-          if (lane >= d) upto += other;
+    if (t > 0.f && finite(m)) {
+      auto mine_of = [&](int s0) {
+        if (s0 + lane >= p.parts) return 0.0;
+        return segment_sum(s0 ? segments[(int64_t)a * p.parts + s0 + lane] : one, m);
+      };
+      double total = 0.0;
+      for (int s0 = 0; s0 < p.parts; s0 += 64) total += mine_of(s0);
+      total = wave_sum64(total);
+      if (total > 0.0) {
+        // the first segment whose running sum passes the drawn number, or the last that has any weight
+        const double target = (double)p.sample[b] * total;
+        double before = 0.0;
+        for (int s0 = 0; s0 < p.parts; s0 += 64) {
+          const double mine = mine_of(s0), upto = before + sum_up_to(mine, lane);
+          const uint64_t passes = __ballot(mine > 0.0 && upto > target), some = __ballot(mine > 0.0);
+          const int l = passes ? __builtin_ctzll(passes) : some ? 63 - __builtin_clzll(some) : -1;
+          if (l >= 0) {
+            at = s0 + l;
+            if (lane == l) target_at = target - (upto - mine);
+          }
+          if (passes) break;
+          before = __shfl(upto, 63);
         }
-        upto += before;
-        const uint64_t passes = __ballot(mine > 0.0 && upto > target), some = __ballot(mine > 0.0);
-        const int l = passes ? __builtin_ctzll(passes) : some ? 63 - __builtin_clzll(some) : -1;
-        if (l >= 0) {
-          at = s0 + l;
-          if (lane == l) target_at = target - (upto - mine);
-        }
-        if (passes) break;
-        before = __shfl(upto, 63);
       }
     }
     if (lane == 0) {
       segment_at = at;
-      found = key;
+      row_key_at = key;
     }
   }
   __syncthreads();
-  int token = winner_index(found);
-  if (segment_at >= 0) {
-    // relative to the row's maximum, as the sums before; each lane takes consecutive elements
-    const float m = key_value(found);
-    const int first = segment_at * kVerifySegment + (int)threadIdx.x * kVerifyPerLane;
-    const int end = min(p.vocab, first + kVerifyPerLane);
-    double w[kVerifyPerLane], mine = 0.0;
+  const uint64_t key = row_key_at;
+  if (segment_at < 0) {
+    if (threadIdx.x == 0) tokens[a] = winner_index(key);
+    return;
+  }
+  // the segment's weights, relative to the row's maximum as the sums before; each lane takes consecutive elements
+  const float m = key_value(key);
+  const int first = segment_at * kVerifySegment + (int)threadIdx.x * kVerifyPerLane;
+  const int end = min(p.vocab, segment_at * kVerifySegment + kVerifySegment);
+  float x[kVerifyPerLane];
+  some_logits<kDtype, kVerifyPerLane>(row, first, end, x);
+  double w[kVerifyPerLane], mine = 0.0;
+#pragma unroll
+  for (int i = 0; i < kVerifyPerLane; ++i) {
+    w[i] = first + i == draft ? 0.0 : weight_of(x[i], m, c);
+    mine += w[i];
+  }
+  double upto = sum_up_to(mine, lane);
+  if (lane == 63) wave_sums[wave] = upto;
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k) upto += k < wave ? wave_sums[k] : 0.0;
+  const uint64_t passes = __ballot(mine > 0.0 && upto > target_at), some = __ballot(mine > 0.0);
+  if (lane == 0) {
+    passes_at[wave] = passes ? __builtin_ctzll(passes) : -1;
+    some_at[wave] = some ? 63 - __builtin_clzll(some) : -1;
+  }
+  __syncthreads();
+  int chosen = -1;   // the first lane whose running sum passes, or the last that has any weight
+#pragma unroll
+  for (int k = 0; k < kWaves; ++k)
+    if (some_at[k] >= 0) chosen = 64 * k + some_at[k];
+#pragma unroll
+  for (int k = kWaves - 1; k >= 0; --k)
+    if (passes_at[k] >= 0) chosen = 64 * k + passes_at[k];
+  if ((int)threadIdx.x == chosen) {
+    double sum = upto - mine;
+    int last = 0, at = -1;
 #pragma unroll
     for (int i = 0; i < kVerifyPerLane; ++i) {
-      w[i] = first + i < end && first + i != draft ? weight_of(logit<kDtype>(row, first + i), m, inv_t) : 0.0;
-      mine += w[i];
-    }
-    lane_sums[threadIdx.x] = mine;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      double upto = 0.0;
-      int at = 0, last = 0;
-      for (; at < kVerifyLanes; ++at) {
-        if (lane_sums[at] > 0.0) {
-          last = at;
-          if (upto + lane_sums[at] > target_at) break;
-        }
-        if (at + 1 < kVerifyLanes) upto += lane_sums[at];
+      sum += w[i];
+      if (w[i] > 0.0) {
+        last = i;
+        if (at < 0 && sum > target_at) at = i;
       }
-      if (at == kVerifyLanes) {
-        at = last;
-        target_at = __builtin_inf();
-      } else {
-        target_at -= upto;
-      }
-      segment_at = at;
     }
-    __syncthreads();
-    if ((int)threadIdx.x == segment_at) {
-      double upto = 0.0;
-      int last = 0, at = -1;
-#pragma unroll
-      for (int i = 0; i < kVerifyPerLane; ++i) {
-        upto += w[i];
-        if (w[i] > 0.0) {
-          last = i;
-          if (at < 0 && upto > target_at) at = i;
-        }
-      }
-      rejected = first + (at < 0 ? last : at);
-    }
-    __syncthreads();
-    token = rejected;
+    tokens[a] = first + (at < 0 ? last : at);
   }
-  for (int k = threadIdx.x; k <= p.max_drafts; k += kVerifyLanes)
-    tokens[k] = k < a ? p.drafts[b * p.draft_stride + k] : k == a ? (int64_t)token : -1;
-  if (threadIdx.x == 0) p.out_counts[b] = a + 1;
 }
 
 }  // namespace arctic
