@@ -1,6 +1,6 @@
 // Verification of drafted tokens against the target model's logits, gfx950.
 //
-// Two launches.  The first walks every row of logits in segments, one workgroup each: the segment's argmax and, relative
+// Two launches.  The first walks every row of logits in segments, one wave each: the segment's argmax and, relative
 // to its maximum, the sum of its weights exp((x - m) / T) without the drafted token's.  The second, one workgroup per
 // request, joins the segments of the request's rows, runs down its drafts to the first that is not accepted, finds the
 // segment in which the running sum passes the drawn number and walks that segment alone.
@@ -19,13 +19,17 @@
 
 namespace arctic {
 
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
 constexpr int kVerifyLanes = 256;
-constexpr int kVerifyPerLane = 16;
-constexpr int kVerifySegment = kVerifyLanes * kVerifyPerLane;
+constexpr int kVerifySegment = 2048;
+constexpr int kVerifyPerLane = kVerifySegment / kVerifyLanes;   // where a workgroup walks a segment
 
 struct VerifySegment {
   double sum;     // of the weights relative to the segment's maximum, without the draft's
-  uint64_t key;   // the segment's argmax
+  uint64_t key;   // the segment's maximum, and its argmax where no token is drawn: of a temperature that is not positive, and
+                  // of a maximum that is not finite
 };
 
 struct VerifyParams {
@@ -37,6 +41,7 @@ struct VerifyParams {
   VerifySegment *segments;   // [batch][max_drafts + 1][parts]
   int64_t row_stride_bytes, draft_stride, accept_stride, num_rows;
   int vocab, max_drafts, parts;
+  uint32_t places;   // batch * (max_drafts + 1)
   Divisor by_parts, by_places;   // by_places: max_drafts + 1
 };
 
@@ -47,32 +52,51 @@ __device__ __forceinline__ float logit(const char *row, int i) {
   return kDtype == ARCTIC_DTYPE_BF16 ? BF16::lo(bits) : F16::lo(bits);
 }
 
-// kPerLane consecutive logits from `first` on, -inf for those at `end` and beyond; whole 16-byte chunks at a time, rows may
-// start anywhere.
-template <int kDtype, int kCount>
-__device__ __forceinline__ void some_logits(const char *row, int first, int end, float (&x)[kCount]) {
+// kChunks chunks of 16 bytes of logits, `stride` logits from one to the next, from `first` on; rows may start anywhere.
+// -inf for logits at `end` and beyond, where the wave's chunks reach it (`last`: the wave's last logit and one).  Returns
+// their sum (two 16-bit ones to an instruction): NaN if there is a NaN among them, or infinities of both signs.
+template <int kDtype, int kChunks>
+__device__ __forceinline__ float some_logits(const char *row, int first, int stride, int last, int end,
+                                            float (&x)[kChunks][kDtype == ARCTIC_DTYPE_F32 ? 4 : 8]) {
   constexpr int kElt = kDtype == ARCTIC_DTYPE_F32 ? 4 : 2, kPerChunk = 16 / kElt;
-  if (first + kCount <= end) {
-    uint4 raw[kCount / kPerChunk];
+  float sum = 0.f;
+  if (last <= end) {
+    uint4 raw[kChunks];
 #pragma unroll
-    for (int i = 0; i < kCount / kPerChunk; ++i) raw[i] = load16<true>(row + (int64_t)(first + i * kPerChunk) * kElt);
+    for (int i = 0; i < kChunks; ++i) raw[i] = load16<true>(row + (int64_t)(first + i * stride) * kElt);
 #pragma unroll
-    for (int i = 0; i < kCount / kPerChunk; ++i) {
+    for (int i = 0; i < kChunks; ++i) {
       if constexpr (kDtype == ARCTIC_DTYPE_F32) {
-        x[4 * i] = __uint_as_float(raw[i].x), x[4 * i + 1] = __uint_as_float(raw[i].y);
-        x[4 * i + 2] = __uint_as_float(raw[i].z), x[4 * i + 3] = __uint_as_float(raw[i].w);
+        x[i][0] = __uint_as_float(raw[i].x), x[i][1] = __uint_as_float(raw[i].y);
+        x[i][2] = __uint_as_float(raw[i].z), x[i][3] = __uint_as_float(raw[i].w);
+        sum += (x[i][0] + x[i][1]) + (x[i][2] + x[i][3]);
       } else {
-        float f[8];
-        if constexpr (kDtype == ARCTIC_DTYPE_BF16) unpack8<BF16>(raw[i], f);
-        else unpack8<F16>(raw[i], f);
+        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[8 * i + j] = f[j];
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (kDtype == ARCTIC_DTYPE_BF16) {
+            const bf16x2 ones = {(__bf16)1.f, (__bf16)1.f};
+            sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w[j]), ones, sum, false);
+            x[i][2 * j] = BF16::lo(w[j]), x[i][2 * j + 1] = BF16::hi(w[j]);
+          } else {
+            const f16x2 ones = {(_Float16)1.f, (_Float16)1.f};
+            sum = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, w[j]), ones, sum, false);
+            x[i][2 * j] = F16::lo(w[j]), x[i][2 * j + 1] = F16::hi(w[j]);
+          }
+        }
       }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) x[i] = first + i < end ? logit<kDtype>(row, first + i) : -__builtin_inff();
+    for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+      for (int j = 0; j < kPerChunk; ++j) {
+        const int at = first + i * stride + j;
+        x[i][j] = at < end ? logit<kDtype>(row, at) : -__builtin_inff();
+        sum += at < end ? x[i][j] : 0.f;
+      }
   }
+  return sum;
 }
 
 // The value that a key was made of (NaN for any NaN, -inf for no key).
@@ -83,14 +107,11 @@ __device__ __forceinline__ float key_value(uint64_t key) {
   return __uint_as_float(o ^ ((o & 0x80000000u) ? 0x80000000u : 0xffffffffu));
 }
 
-// 2^((x - m) c) in fp64, relative error 2e-14, for (x - m) c <= 0; 0 below 2^-1074 and for x = -inf whatever c is.
-// t = n + f with n whole (found by adding 1.5 2^52, whose last bit is worth 1) and |f| <= 1/2, 2^f by its Chebyshev
-// interpolation of degree 9 there.
-__device__ __forceinline__ double weight_of(double x, double m, double c) {
-  const double t = fmax((x - m) * c, -1100.0);
-  const double shifted = t + 6755399441055744.0;
-  const int n = (int)(uint32_t)__double_as_longlong(shifted);
-  const double f = t - (shifted - 6755399441055744.0);
+// 2^((x - m) c) in fp64, relative error 2e-14, for x <= m: with (x - m) c = n + f, n whole (found by adding 1.5 2^52, whose
+// last bit is worth 1) and |f| <= 1/2, 2^f by its Chebyshev interpolation of degree 9 there.  (One product and difference in
+// place of the difference and the product would do for temperatures about 1; at 1e-30 it leaves x = m with a weight that is
+// not 1.)
+__device__ __forceinline__ double power_of_fraction(double f) {
   double v = 0x1.b6571ea79d565p-24;
   v = fma(v, f, 0x1.63ef969b0e64ep-20);
   v = fma(v, f, 0x1.ffcb7677a5f5cp-17);
@@ -100,18 +121,45 @@ __device__ __forceinline__ double weight_of(double x, double m, double c) {
   v = fma(v, f, 0x1.c6b08d7044115p-5);
   v = fma(v, f, 0x1.ebfbdff8149f2p-3);
   v = fma(v, f, 0x1.62e42fefa39f7p-1);
-  v = fma(v, f, 0x1.000000000003dp+0);
-  return __builtin_amdgcn_ldexp(v, n);
+  return fma(v, f, 0x1.000000000003dp+0);
 }
+constexpr double kWholeBits = 6755399441055744.0;   // 1.5 2^52
+// for any x, -inf among them, and any c: 0 below 2^-1074
+__device__ __forceinline__ double weight_of(double x, double m, double c) {
+  const double t = fmax((x - m) * c, -1100.0);
+  const double shifted = t + kWholeBits;
+  return __builtin_amdgcn_ldexp(power_of_fraction(t - (shifted - kWholeBits)), (int)(uint32_t)__double_as_longlong(shifted));
+}
+// where (x - m) c is known to be above -1020: the exponent takes n as it is.  (fp64 maxima, scalings and conversions run at a
+// fraction of the products' rate.)
+__device__ __forceinline__ double weight_in_range(double x, double m, double c) {
+  const double d = x - m, shifted = fma(d, c, kWholeBits);
+  const double v = power_of_fraction(fma(d, c, -(shifted - kWholeBits)));
+  return __hiloint2double(__double2hiint(v) + ((int)(uint32_t)__double_as_longlong(shifted) << 20), __double2loint(v));
+}
+// What a segment's 2048 weights below 2^-1001, logits at the end of that range and beyond, may add up to counts as none.
+constexpr double kLeastSum = 0x1p-980;
 // c for temperature t: log2(e) / t
 __device__ __forceinline__ double per_unit(float t) { return 1.4426950408889634074 / (double)t; }
 
 __device__ __forceinline__ bool finite(float v) { return fabsf(v) < __builtin_inff(); }
 
+// The same sum in every lane: inside the rows of 16 lanes by DPP, then the four rows'.
+template <int kCtrl>
+__device__ __forceinline__ double dpp_add64(double v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), kCtrl, 0xf, 0xf, true);
+  const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), kCtrl, 0xf, 0xf, true);
+  return v + __hiloint2double(hi, lo);
+}
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), lane), __builtin_amdgcn_readlane(__double2loint(v), lane));
+}
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  return v;
+  v = dpp_add64<0xB1>(v);    // quad_perm [1,0,3,2]
+  v = dpp_add64<0x4E>(v);    // quad_perm [2,3,0,1]
+  v = dpp_add64<0x141>(v);   // row_half_mirror
+  v = dpp_add64<0x140>(v);   // row_mirror
+  return (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
 }
 // the sum of a lane's value and those of the lanes before it
 __device__ __forceinline__ double sum_up_to(double v, int lane) {
@@ -130,80 +178,98 @@ __device__ __forceinline__ int drafts_of(const VerifyParams &p, int b, int64_t *
   return first < 0 || end <= first ? -1 : (int)min((int64_t)p.max_drafts, end - first - 1);
 }
 
+// A segment per wave: nothing is shared and nothing waited for but the logits, 64 or 128 bytes a lane.  (Segments of 4096
+// by workgroups of 256 lanes, with three barriers, took 26.6 us where this takes 24 of 64 requests' 219 rows of 128256
+// bf16 logits.)
 template <int kDtype>
 __global__ __launch_bounds__(kVerifyLanes) void verify_segments_kernel(const VerifyParams p) {
-  constexpr int kWaves = kVerifyLanes / 64, kChunk = kDtype == ARCTIC_DTYPE_F32 ? 4 : 8, kLoads = kVerifyPerLane / kChunk;
-  __shared__ uint64_t keys[kWaves];
-  __shared__ double sums[kWaves];
-  const uint32_t place = p.by_parts.quotient(blockIdx.x);   // b * (max_drafts + 1) + k
-  const int part = (int)(blockIdx.x - place * (uint32_t)p.parts);
+  constexpr int kChunk = kDtype == ARCTIC_DTYPE_F32 ? 4 : 8, kLoads = kVerifySegment / 64 / kChunk;
+  const uint32_t unit = blockIdx.x * (kVerifyLanes / 64) + (uint32_t)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const uint32_t place = p.by_parts.quotient(unit);   // b * (max_drafts + 1) + k
+  const int part = (int)(unit - place * (uint32_t)p.parts);
+  if (place >= p.places) return;
   const int b = (int)p.by_places.quotient(place), k = (int)(place - (uint32_t)b * (uint32_t)(p.max_drafts + 1));
   int64_t start;
   const int n = drafts_of(p, b, &start);
   if (k > n) return;
   const char *row = p.logits + (start + k) * p.row_stride_bytes;
-  const int lane = threadIdx.x, first = part * kVerifySegment, end = min(p.vocab, first + kVerifySegment);
+  const int lane = threadIdx.x & 63, first = part * kVerifySegment, end = min(p.vocab, first + kVerifySegment);
   // neighbouring lanes take neighbouring chunks
   float x[kLoads][kChunk];
-#pragma unroll
-  for (int i = 0; i < kLoads; ++i) some_logits<kDtype, kChunk>(row, first + (i * kVerifyLanes + lane) * kChunk, end, x[i]);
+  const float probe = some_logits<kDtype, kLoads>(row, first + lane * kChunk, 64 * kChunk, first + kVerifySegment, p.vocab, x);
   const float t = p.temperatures ? p.temperatures[b] : 1.f;
   const int64_t draft = k < n ? p.drafts[b * p.draft_stride + k] : -1;
   // the lane's maximum; a NaN is above every number, and is looked for only where a sum says that there may be one
-  float top = -__builtin_inff(), probe = 0.f;
+  float top = -__builtin_inff();
 #pragma unroll
   for (int i = 0; i < kLoads; ++i)
 #pragma unroll
-    for (int j = 0; j < kChunk; ++j) {
-      top = fmaxf(top, x[i][j]);
-      probe += x[i][j];
-    }
-  if (probe != probe) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-#pragma unroll
-      for (int j = 0; j < kChunk; ++j)
-        if (x[i][j] != x[i][j]) top = __builtin_nanf("");
-  }
-  // the segment's maximum, then the lowest index that has it
-  const uint32_t mine = (uint32_t)(winner_key(top, 0) >> 32), wave_top = wave_max<4>(mine);
-  if ((lane & 63) == 0) keys[lane >> 6] = wave_top;
-  __syncthreads();
-  const uint32_t all_top = max(max((uint32_t)keys[0], (uint32_t)keys[1]), max((uint32_t)keys[2], (uint32_t)keys[3]));
-  const float m = key_value((uint64_t)all_top << 32);
-  int at = 0x7fffffff;
-  if (mine == all_top) {
-#pragma unroll
-    for (int i = kLoads - 1; i >= 0; --i)
-#pragma unroll
-      for (int j = kChunk - 1; j >= 0; --j) {
-        const int index = first + (i * kVerifyLanes + lane) * kChunk + j;
-        if (index < end && (x[i][j] == m || (m != m && x[i][j] != x[i][j]))) at = index;
-      }
-  }
-  const uint32_t lowest = ~wave_max<4>(~(uint32_t)at);
-  double sum = 0.0;
-  if (t > 0.f && finite(m)) {
-    const double c = per_unit(t);
+    for (int j = 0; j < kChunk; j += 2) top = fmaxf(fmaxf(top, x[i][j]), x[i][j + 1]);
+  // (a value by another name: what is asked of it must not be worked out beforehand and thrown away)
+  auto renamed = [](float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+  };
+  if (__any(probe != probe)) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
 #pragma unroll
       for (int j = 0; j < kChunk; ++j) {
-        const double w = weight_of(x[i][j], m, c);
-        sum += first + (i * kVerifyLanes + lane) * kChunk + j == draft ? 0.0 : w;
+        const float v = renamed(x[i][j]);
+        if (v != v) top = __builtin_nanf("");
       }
   }
-  sum = wave_sum64(sum);
-  __syncthreads();
-  if ((lane & 63) == 0) {
-    keys[lane >> 6] = lowest;
-    sums[lane >> 6] = sum;
+  const uint32_t mine = (uint32_t)(winner_key(top, 0) >> 32), all_top = wave_max<4>(mine);
+  const float m = key_value((uint64_t)all_top << 32);
+  const bool drawn = t > 0.f && finite(m);
+  uint32_t not_lowest = 0;   // the complement of the lowest index that has the maximum, where it is asked for
+  if (!drawn) {
+    int at = 0x7fffffff;
+    if (mine == all_top) {
+#pragma unroll
+      for (int i = kLoads - 1; i >= 0; --i)
+#pragma unroll
+        for (int j = kChunk - 1; j >= 0; --j) {
+          const int index = first + (i * 64 + lane) * kChunk + j;
+          const float v = renamed(x[i][j]);
+          if (index < end && (v == m || (m != m && v != v))) at = index;
+        }
+    }
+    not_lowest = wave_max<4>(~(uint32_t)at);
   }
-  __syncthreads();
-  if (lane == 0) {
-    const uint32_t index = min(min((uint32_t)keys[0], (uint32_t)keys[1]), min((uint32_t)keys[2], (uint32_t)keys[3]));
-    p.segments[blockIdx.x] = {(sums[0] + sums[1]) + (sums[2] + sums[3]), (uint64_t)all_top << 32 | ~index};
+  double sum = 0.0;
+  if (drawn) {
+    const double c = per_unit(t);
+    if (draft >= first && draft < end) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j)
+          if (first + (i * 64 + lane) * kChunk + j == draft) x[i][j] = -__builtin_inff();
+    }
+    // Below `lowest` weights are as good as none.  Where the type's steps are too wide to say so (tiny temperatures), or its
+    // range too narrow (huge ones), every weight is looked at.
+    const float lowest = (float)((double)m - 1010.0 / c);
+    const double span = ((double)m - (double)lowest) * c;
+    if (span > 1001.0 && span < 1020.0) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) {
+          float v;   // (no NaN is left here that fmaxf would first have to quieten)
+          asm("v_max_f32 %0, %1, %2" : "=v"(v) : "v"(x[i][j]), "v"(lowest));
+          sum += weight_in_range(v, m, c);
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i)
+#pragma unroll
+        for (int j = 0; j < kChunk; ++j) sum += weight_of(x[i][j], m, c);
+    }
+    sum = wave_sum64(sum);
+    sum = sum < kLeastSum ? 0.0 : sum;
   }
+  if (lane == 0) p.segments[unit] = {sum, (uint64_t)all_top << 32 | not_lowest};
 }
 
 template <int kDtype>
@@ -304,20 +370,22 @@ __global__ __launch_bounds__(kVerifyLanes) void verify_requests_kernel(const Ver
   }
   __syncthreads();
   const uint64_t key = row_key_at;
+  // the argmax: of a row with a distribution in which no other token has any weight the rejected draft
+  const int64_t otherwise = t > 0.f && finite(key_value(key)) ? draft : (int64_t)winner_index(key);
   if (segment_at < 0) {
-    if (threadIdx.x == 0) tokens[a] = winner_index(key);
+    if (threadIdx.x == 0) tokens[a] = otherwise;
     return;
   }
   // the segment's weights, relative to the row's maximum as the sums before; each lane takes consecutive elements
   const float m = key_value(key);
   const int first = segment_at * kVerifySegment + (int)threadIdx.x * kVerifyPerLane;
-  const int end = min(p.vocab, segment_at * kVerifySegment + kVerifySegment);
-  float x[kVerifyPerLane];
-  some_logits<kDtype, kVerifyPerLane>(row, first, end, x);
+  constexpr int kChunk = kDtype == ARCTIC_DTYPE_F32 ? 4 : 8;
+  float x[kVerifyPerLane / kChunk][kChunk];
+  some_logits<kDtype, kVerifyPerLane / kChunk>(row, first, kChunk, segment_at * kVerifySegment + kVerifySegment, p.vocab, x);
   double w[kVerifyPerLane], mine = 0.0;
 #pragma unroll
   for (int i = 0; i < kVerifyPerLane; ++i) {
-    w[i] = first + i == draft ? 0.0 : weight_of(x[i], m, c);
+    w[i] = first + i == draft ? 0.0 : weight_of(x[i / kChunk][i % kChunk], m, c);
     mine += w[i];
   }
   double upto = sum_up_to(mine, lane);
@@ -338,7 +406,9 @@ __global__ __launch_bounds__(kVerifyLanes) void verify_requests_kernel(const Ver
 #pragma unroll
   for (int k = kWaves - 1; k >= 0; --k)
     if (passes_at[k] >= 0) chosen = 64 * k + passes_at[k];
-  if ((int)threadIdx.x == chosen) {
+  if (chosen < 0) {   // (no weight here after all)
+    if (threadIdx.x == 0) tokens[a] = otherwise;
+  } else if ((int)threadIdx.x == chosen) {
     double sum = upto - mine;
     int last = 0, at = -1;
 #pragma unroll
@@ -410,12 +480,13 @@ extern "C" int arctic_verify_drafts(int64_t *out_tokens, int64_t *out_counts, co
   p.vocab = vocab_size;
   p.max_drafts = max_drafts;
   p.parts = (int)parts;
+  p.places = (uint32_t)(batch * (max_drafts + 1));
   p.by_parts = Divisor((uint32_t)parts);
   p.by_places = Divisor((uint32_t)(max_drafts + 1));
   hipStream_t s = (hipStream_t)stream;
 #define ARCTIC_VERIFY(DTYPE)                                                                   \
   do {                                                                                         \
-    launch(verify_segments_kernel<DTYPE>, dim3((unsigned)grid), kVerifyLanes, s, p);           \
+    launch(verify_segments_kernel<DTYPE>, dim3((unsigned)((grid + 3) / 4)), kVerifyLanes, s, p); \
     launch(verify_requests_kernel<DTYPE>, dim3((unsigned)batch), kVerifyLanes, s, p);          \
   } while (0)
   if (dtype == ARCTIC_DTYPE_F32) ARCTIC_VERIFY(ARCTIC_DTYPE_F32);
