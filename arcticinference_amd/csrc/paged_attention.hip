@@ -252,6 +252,12 @@ static bool few_takes(const AttentionParams &p) {
   return wide % 16 == 0 && p.key_token < (1 << 26) && p.value_token < (1 << 26) && p.num_blocks > 0 && p.max_blocks > 0;
 }
 
+// ... and in the kernel for many tokens a block's stride and what lies inside one have 32 bits.
+static bool many_takes(const AttentionParams &p) {
+  return few_takes(p) && p.key_block <= 0xffffffffLL && p.value_block <= 0xffffffffLL &&
+         p.key_token * p.block_size <= 0xffffffffLL && p.value_token * p.block_size <= 0xffffffffLL;
+}
+
 static int64_t few_bytes(const FewShape &f, int64_t batch, int64_t new_tokens, int num_heads, int head_size) {
   return f.least == 0 ? 0 : new_tokens * num_heads * 2 * f.workers * ((int64_t)head_size + 2) * 4 + batch * (int64_t)sizeof(int2);
 }
@@ -264,21 +270,22 @@ static bool many_shape(ManyShape &f, int64_t batch, int64_t new_tokens, int64_t 
   if (dtype == ARCTIC_DTYPE_F32 || c.head_size > 256 || c.head_size % (c.kv_cache_dtype == ARCTIC_KV_AUTO ? 8 : 16)) return false;
   const int64_t group = num_heads / c.num_kv_heads, rows = total_tokens * group;
   f.padded = c.head_size <= 64 ? 64 : c.head_size <= 128 ? 128 : 256;
-  f.waves = f.padded == 256 || rows * c.num_kv_heads < 256 * 256 ? 4 : 8;
-  const int64_t tile = 32 * f.waves;
-  f.per_sequence = (int)std::min<int64_t>((new_tokens * group + tile - 1) / tile, 0x7fffffff);
-  f.slots = new_tokens ? batch * f.per_sequence : rows / tile + batch;
-  // The row tiles that there are for sure: rows / tile; splits where they leave CUs idle.
-  const int64_t units = std::max<int64_t>(1, rows / tile) * c.num_kv_heads;
-  const int64_t tiles = (most_tiles(max_seq_len, tile / group + 1, window, num_sinks) + 1) / 2;
-  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(256 / units, (tiles + 7) / 8));
+  f.per_sequence = (int)std::min<int64_t>((new_tokens * group + kManyRows - 1) / kManyRows, 0x7fffffff);
+  f.slots = new_tokens ? batch * f.per_sequence : rows / kManyRows + batch;
+  // The row tiles that there are for sure: rows / kManyRows.  A CU has two workgroups at a time, and those of long and short
+  // sequences, of a sequence's first and last rows differ: splits that make four for a CU even them out (two chunks of up to
+  // 512 tokens behind up to 24000 keys, 64 heads over 8: 647 us; two for a CU 705, eight 632 with twice the workspace).  A
+  // split of fewer than 8 tiles is not worth the join.
+  const int64_t units = std::max<int64_t>(1, rows / kManyRows) * c.num_kv_heads;
+  const int64_t keys = many_keys(f.padded), tiles = (most_tiles(max_seq_len, kManyRows / group + 1, window, num_sinks) * 32 + keys - 1) / keys;
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(1024 / units, (tiles + 7) / 8));
   f.tiles_per_split = (int)((tiles + splits - 1) / splits);
   f.splits = (int)((tiles + f.tiles_per_split - 1) / f.tiles_per_split);
   return f.slots * f.splits * c.num_kv_heads <= 0x7fffffffLL;
 }
 
 static int64_t many_bytes(const ManyShape &f, int num_kv_heads, int head_size) {
-  return f.splits == 1 ? 0 : f.slots * num_kv_heads * f.splits * 32 * f.waves * ((int64_t)head_size + 2) * 4;
+  return f.splits == 1 ? 0 : f.slots * num_kv_heads * f.splits * kManyRows * ((int64_t)head_size + 2) * 4;
 }
 
 static int workspace_error(const char *fn, int64_t need) {
@@ -300,7 +307,7 @@ static int run_many(const char *fn, const AttentionParams &p, const ManyShape &f
   mp.by_per_sequence = Divisor((uint32_t)std::max(1, f.per_sequence));
   mp.by_group = Divisor((uint32_t)p.group);
   mp.partial = need ? (float *)workspace : nullptr;
-  mp.statistics = need ? mp.partial + f.slots * p.kv_heads * f.splits * 32 * f.waves * p.head_size : nullptr;
+  mp.statistics = need ? mp.partial + f.slots * p.kv_heads * f.splits * kManyRows * p.head_size : nullptr;
   if (dtype == ARCTIC_DTYPE_BF16) many_launch_bf16(mp, f, kv, s);
   else many_launch_f16(mp, f, kv, s);
   return check_launch(fn);
@@ -348,7 +355,7 @@ extern "C" int arctic_paged_attention(void *out, const void *query, const arctic
   FewShape f;
   ManyShape m;
   if ((int64_t)new_tokens * p.group > kMostFewRows) {
-    if (few_takes(p) && many_shape(m, batch, new_tokens, p.total_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype))
+    if (many_takes(p) && many_shape(m, batch, new_tokens, p.total_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype))
       return run_many(fn, p, m, dtype, cache->kv_cache_dtype, workspace, workspace_bytes, (hipStream_t)stream);
   } else if (few_takes(p) && few_shape(f, batch, new_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype)) {
     const int64_t need = few_bytes(f, batch, new_tokens, num_heads, cache->head_size);
@@ -403,7 +410,7 @@ extern "C" int arctic_paged_attention_ragged(void *out, const void *query, const
   if (max_seq_len < 0) return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: max_seq_len must not be negative", fn);
   p.query_start = query_start;
   ManyShape m;
-  if (few_takes(p) && many_shape(m, batch, 0, total_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype))
+  if (many_takes(p) && many_shape(m, batch, 0, total_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype))
     return run_many(fn, p, m, dtype, cache->kv_cache_dtype, workspace, workspace_bytes, (hipStream_t)stream);
   return run_attention(fn, p, dtype, cache->kv_cache_dtype, (hipStream_t)stream);
 }

@@ -102,7 +102,7 @@ def attention_in_64_bits(case, window=None, sinks=0):
                 w = torch.softmax(s, 0)
                 o = w @ v[:, h // group]
                 spread = w @ v[:, h // group].abs()
-                terms = (k[:, h // group].abs() @ q.abs()).max() * case["scale"]
+                terms = (k[:, h // group].abs() @ q.abs()).max() * abs(case["scale"])   # |scale| sum |q k| bounds every partial sum
                 fine = 2.0 ** -24 * (2 * (size + 4) * terms + 6 * s.abs().max() + 2 * s.numel() + 32)
                 out[first + i, h] = o
                 bound[first + i, h] = last * o.abs() + half * (spread + o.abs()) + fine * (spread + o.abs()) + \

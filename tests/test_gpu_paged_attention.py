@@ -241,6 +241,21 @@ def test_a_peak_in_any_split(ops):
         check(ops, c)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("slope", [0.004, 0.04, 0.4, -0.04])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_that_rise_and_fall_with_the_position(ops, dtype, slope, sign):
+    """The running maximum moves a little or a lot with every tile, or never again."""
+    c = make_attention_case(lengths=[700, 333], new=[70, 70], heads=4, kv_heads=2, size=64, dtype=dtype, seed=31, std=0.25, device=DEV)
+    c["query"] += 0.5
+    c["scale"] *= sign
+    for b, n in enumerate(c["lengths"]):
+        j = torch.arange(n, device=DEV)
+        at = c["table"][b].long()[j // 16], j % 16
+        c["key"][at] += (sign * slope * j).to(dtype)[:, None, None]
+    check(ops, c)
+
+
 def test_no_sequence_and_no_query(ops):
     c = make_attention_case(lengths=[30], new=[1], heads=4, kv_heads=2, size=64, seed=24, device=DEV)
     empty = torch.empty(0, dtype=torch.int32, device=DEV)
