@@ -12,7 +12,7 @@
 // waves that share K and V (10 % for windows, even elsewhere: they wait for each other); 64 rows a wave, one wave a SIMD, each
 // LDS read feeding two products (272 us for 187); a wave's weights computed in the middle of its own products (212 for 203).
 // Four prompts of up to 2500 tokens, 32 heads over 8 x 128: 187 us, 730 TFLOP/s; two chunks of up to 512 tokens behind up to
-// 24000 fp8 keys, 64 heads over 8 x 128: 647 us, 850 TFLOP/s.
+// 24000 fp8 keys, 64 heads over 8 x 128: 640 us, 860 TFLOP/s.
 #pragma once
 
 #include "paged_attention_few.hpp"
@@ -199,9 +199,10 @@ __global__ __launch_bounds__(64 * kManyWaves, kPadded > 128 ? 1 : 2) void attent
       value_in[i] = *(const ARCTIC_GLOBAL u32x4 *)(value_from + value_at);
     }
   };
-  // chunk of row k, where it lies: K's readers take one chunk of 32 rows, V's four chunks of four rows
-  auto key_place = [](int k, int chunk) { return k * kChunks + (chunk ^ (kChunks == 8 ? k >> 1 & 7 : k & 15)); };
-  auto value_place = [](int k, int chunk) { return k * kChunks + (chunk ^ (kChunks == 8 ? (k >> 1 & 1) << 2 : (k & 3) << 2)); };
+  // Chunk of row k, where it lies.  K's readers take one chunk of 32 rows, V's four chunks of four rows, and the writers of an
+  // fp8 cache every other chunk of two to four rows, or of one that passes all banks.
+  auto key_place = [](int k, int chunk) { return k * kChunks + (chunk ^ chunk >> 4 ^ (kChunks == 8 ? k >> 1 & 7 : k & 15)); };
+  auto value_place = [](int k, int chunk) { return k * kChunks + (chunk ^ chunk >> 4 ^ (kChunks == 8 ? (k >> 1 & 1) * 5 : (k & 3) << 2 | (k & 1))); };
   // Into LDS; with `look`, looking for values that are infinite or NaN.
   auto keep = [&](int buffer, bool look) {
     bool found = false;
