@@ -199,10 +199,10 @@ __global__ __launch_bounds__(64 * kManyWaves, kPadded > 128 ? 1 : 2) void attent
       value_in[i] = *(const ARCTIC_GLOBAL u32x4 *)(value_from + value_at);
     }
   };
-  // Chunk of row k, where it lies.  K's readers take one chunk of 32 rows, V's four chunks of four rows, and the writers of an
-  // fp8 cache every other chunk of two to four rows, or of one that passes all banks.
-  auto key_place = [](int k, int chunk) { return k * kChunks + (chunk ^ chunk >> 4 ^ (kChunks == 8 ? k >> 1 & 7 : k & 15)); };
-  auto value_place = [](int k, int chunk) { return k * kChunks + (chunk ^ chunk >> 4 ^ (kChunks == 8 ? (k >> 1 & 1) * 5 : (k & 3) << 2 | (k & 1))); };
+  // Chunk of row k, where it lies.  K's readers take one chunk of 32 rows, V's four chunks of four rows.  Eight lanes write
+  // at once, of an fp8 cache every other chunk of a row or two: the last bit parts those that would meet within 128 bytes.
+  auto key_place = [](int k, int chunk) { return k * kChunks + (chunk ^ (chunk >> 3 & 1) ^ (kChunks == 8 ? (k >> 1 & 7) ^ (k & 1) : k & 15)); };
+  auto value_place = [](int k, int chunk) { return k * kChunks + (chunk ^ (chunk >> 3 & 1) ^ (kChunks == 8 ? (k >> 1 & 1) << 2 | (k & 1) : (k & 3) << 2)); };
   // Into LDS; with `look`, looking for values that are infinite or NaN.
   auto keep = [&](int buffer, bool look) {
     bool found = false;
