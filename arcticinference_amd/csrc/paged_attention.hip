@@ -223,7 +223,7 @@ static bool few_shape(FewShape &f, int64_t batch, int64_t new_tokens, int num_he
   if (dtype == ARCTIC_DTYPE_F32 || c.head_size > 256 || c.head_size % (c.kv_cache_dtype == ARCTIC_KV_AUTO ? 8 : 16)) return false;
   const int64_t rows = new_tokens * (num_heads / c.num_kv_heads);
   f.padded = c.head_size <= 64 ? 64 : c.head_size <= 128 ? 128 : 256;
-  f.columns = rows <= 16 ? 1 : rows <= 32 || f.padded == 256 ? 2 : 4;
+  f.columns = rows <= 16 ? 1 : rows <= 32 || f.padded > 64 ? 2 : 4;
   const int64_t row_tiles = (rows + 16 * f.columns - 1) / (16 * f.columns);
   f.plain = c.head_size == f.padded && c.block_size % 16 == 0;
   // rows of 128 bytes and less of neighbouring heads are read together
@@ -313,8 +313,16 @@ static int run_many(const char *fn, const AttentionParams &p, const ManyShape &f
   return check_launch(fn);
 }
 
-// Query rows of a key head beyond which the kernel for many tokens is the faster one.
-constexpr int64_t kMostFewRows = 64;
+// Query rows of a key head beyond which the kernel for many tokens is the faster one.  32 heads over 8, few / many tokens, us:
+//                     16 x 2000 keys, 48 rows   48 x 4000, 32 rows   48 x 4000, 48 rows   4 x 32000, 64 rows
+//   128, 16 bits      87 / 34                   176 / 194            235 / 207            164 / 184
+//   128, fp8          63 / 32                   105 / 137            171 / 156            122 / 134
+//   256, 16 bits      165 / 100                 465 / 470            681 / 487            441 / 354
+//   256, fp8          90 / 92                   204 / 417            301 / 443            193 / 324
+//   64, 16 bits       33 / 26                   101 / 108            105 / 117            65 / 104
+static int64_t most_few_rows(const arctic_paged_cache &c) {
+  return c.head_size <= 64 || (c.head_size > 128 && c.kv_cache_dtype != ARCTIC_KV_AUTO) ? 64 : 32;
+}
 
 extern "C" int64_t arctic_paged_attention_workspace_bytes(int64_t batch, int new_tokens, int num_heads,
                                                           const arctic_paged_cache *cache, int64_t max_seq_len,
@@ -326,7 +334,7 @@ extern "C" int64_t arctic_paged_attention_workspace_bytes(int64_t batch, int new
     return 0;
   FewShape f;
   ManyShape m;
-  if (new_tokens * (int64_t)(num_heads / cache->num_kv_heads) > kMostFewRows)
+  if (new_tokens * (int64_t)(num_heads / cache->num_kv_heads) > most_few_rows(*cache))
     return many_shape(m, batch, new_tokens, batch * new_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype)
                ? many_bytes(m, cache->num_kv_heads, cache->head_size)
                : 0;
@@ -354,7 +362,7 @@ extern "C" int arctic_paged_attention(void *out, const void *query, const arctic
   p.by_new = Divisor((uint32_t)new_tokens);
   FewShape f;
   ManyShape m;
-  if ((int64_t)new_tokens * p.group > kMostFewRows) {
+  if ((int64_t)new_tokens * p.group > most_few_rows(*cache)) {
     if (many_takes(p) && many_shape(m, batch, new_tokens, p.total_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype))
       return run_many(fn, p, m, dtype, cache->kv_cache_dtype, workspace, workspace_bytes, (hipStream_t)stream);
   } else if (few_takes(p) && few_shape(f, batch, new_tokens, num_heads, *cache, max_seq_len, window, num_sinks, dtype)) {

@@ -693,7 +693,7 @@ inline void few_launch_plain(const FewParams &p, const FewShape &f, dim3 grid, h
 template <typename T, typename C, int kPadded>
 inline void few_launch_columns(const FewParams &p, const FewShape &f, dim3 grid, hipStream_t s) {
   if (f.columns == 1) return few_launch_plain<T, C, kPadded, 1>(p, f, grid, s);
-  if constexpr (kPadded < 256)
+  if constexpr (kPadded == 64)
     if (f.columns == 4) return few_launch_plain<T, C, kPadded, 4>(p, f, grid, s);
   few_launch_plain<T, C, kPadded, 2>(p, f, grid, s);
 }
