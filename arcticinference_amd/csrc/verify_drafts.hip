@@ -9,6 +9,10 @@
 // one past the drawn number in about one request of a hundred.  They and the weights are therefore held in fp64.  The
 // drafted token is left out of the segments' sums and added where it belongs, so that what remains of a row whose draft
 // holds nearly everything is no difference of nearly equal numbers.
+//
+// The first launch reads the logits once: 160 requests with up to 7 drafts, 128257 fp32 logits a row, 75 us, 5.0 TB/s.  With
+// 16-bit logits the fp64 arithmetic takes longer than the reading: 64 requests with up to 5 drafts, 128256 bf16 logits, 24 us,
+// 2.3 TB/s.  The second is a row of latencies, 6 to 9 us.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
