@@ -28,8 +28,10 @@ __global__ __launch_bounds__(64 * kGeneralWaves) void attention_general_kernel(c
   __shared__ float query[kGeneralMostHead];
   __shared__ float parts[kGeneralWaves][kGeneralMostHead], statistics[kGeneralWaves][2];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const uint32_t token = p.by_heads.quotient(blockIdx.x);
-  const int head = (int)(blockIdx.x - token * (uint32_t)p.heads);
+  const uint32_t unit = blockIdx.y * gridDim.x + blockIdx.x;
+  if (unit >= (uint32_t)p.total_tokens * (uint32_t)p.heads) return;
+  const uint32_t token = p.by_heads.quotient(unit);
+  const int head = (int)(unit - token * (uint32_t)p.heads);
   int b, count, first;
   if (p.query_start) {
     int lo = 0, hi = p.batch;   // the last sequence that starts at or before this row
@@ -229,7 +231,10 @@ static int describe(const char *fn, AttentionParams &p, void *out, const void *q
 
 template <typename Q>
 static void launch_general(const AttentionParams &p, int kv, hipStream_t s) {
-  const dim3 grid((unsigned)(p.total_tokens * p.heads));
+  // a launch has fewer than 2^32 lanes along an axis
+  constexpr int64_t kMost = 1 << 22;
+  const int64_t units = p.total_tokens * p.heads;
+  const dim3 grid((unsigned)std::min(units, kMost), (unsigned)((units + kMost - 1) / kMost));
   if (kv == ARCTIC_KV_AUTO) launch(attention_general_kernel<Q, Q>, grid, 64 * kGeneralWaves, s, p);
   else if (kv == ARCTIC_KV_FP8_E4M3) launch(attention_general_kernel<Q, CacheE4M3>, grid, 64 * kGeneralWaves, s, p);
   else launch(attention_general_kernel<Q, CacheE5M2>, grid, 64 * kGeneralWaves, s, p);
@@ -275,7 +280,8 @@ static bool few_shape(FewShape &f, int64_t batch, int64_t new_tokens, int num_he
     f.least = (int)kLeast;
     f.workers = (int)std::max<int64_t>(1, std::min((kWorkgroups + units - 1) / units, (batch * tiles + kLeast - 1) / kLeast));
   }
-  return units * f.workers <= 0x7fffffffLL && c.num_kv_heads * (int64_t)f.workers <= 0x3fffffffLL;
+  // fewer than 2^32 lanes in either launch (a wave joins a row)
+  return units * f.workers <= 0xffffffLL && batch * new_tokens * num_heads <= 0x3ffffffLL;
 }
 
 // What a lane of few_launch's kernels loads or stores at once, and the 32-bit offsets of a block's 16 tokens.
@@ -315,7 +321,7 @@ static bool many_shape(ManyShape &f, int64_t batch, int64_t new_tokens, int64_t 
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(1024 / units, (tiles + 7) / 8));
   f.tiles_per_split = (int)((tiles + splits - 1) / splits);
   f.splits = (int)((tiles + f.tiles_per_split - 1) / f.tiles_per_split);
-  return f.slots * f.splits * c.num_kv_heads <= 0x7fffffffLL;
+  return f.slots * f.splits * c.num_kv_heads <= 0xffffffLL;   // fewer than 2^32 lanes
 }
 
 static int64_t many_bytes(const ManyShape &f, int num_kv_heads, int head_size) {

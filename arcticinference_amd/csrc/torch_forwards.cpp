@@ -630,6 +630,8 @@ void paged_attention(const at::Tensor &query, const OptTensor &query_start, cons
   TORCH_CHECK(out.scalar_type() == query.scalar_type() && out.sizes() == query.sizes(), fn,
               ": out must have the queries' type and shape");
   TORCH_CHECK(out.stride(d - 1) == 1 || head_size == 1, fn, ": the last dimension of out must be contiguous");
+  for (int64_t i = 0; i < d; ++i)
+    TORCH_CHECK(out.size(i) <= 1 || out.stride(i) != 0, fn, ": out must not be expanded");
   const int64_t batch = ragged ? seq_lens.numel() : query.size(0), new_tokens = d == 4 ? query.size(1) : 1;
   TORCH_CHECK(int_vector(seq_lens, batch), fn, ": seq_lens must be a contiguous int32 tensor with one entry per sequence");
   TORCH_CHECK(block_table.scalar_type() == at::kInt && block_table.dim() == 2 && block_table.size(0) == batch &&

@@ -463,7 +463,7 @@ extern "C" int arctic_verify_drafts(int64_t *out_tokens, int64_t *out_counts, co
     return fail(ARCTIC_ERR_UNSUPPORTED, "%s: logits do not start at a multiple of their element size", fn);
   const int64_t parts = verify_parts(vocab_size);
   const int64_t grid = batch * (max_drafts + 1) * parts;
-  if (grid > 0x7fffffffLL) return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: too many requests for this vocabulary", fn);
+  if (grid > 0x3ffffffLL || batch > 0xffffffLL) return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: too many requests for this vocabulary", fn);
   const int64_t need = arctic_verify_drafts_workspace_bytes(batch, max_drafts, vocab_size, dtype);
   if (!workspace || (uintptr_t)workspace % 8 || workspace_bytes < need)
     return fail(ARCTIC_ERR_INVALID_ARGUMENT, "%s: the workspace must be 8-byte aligned and hold %lld bytes", fn, (long long)need);

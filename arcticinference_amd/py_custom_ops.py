@@ -486,7 +486,8 @@ def paged_attention(
     ``v_scale``, one fp32 each); ``heads`` is a multiple of ``kv_heads``.  ``block_table`` is int32
     ``[batch, blocks]``; an entry outside the cache holds no keys.  ``max_seq_len``, the longest of ``seq_lens`` or more,
     is what the work is split by; results do not depend on it beyond their rounding.  A query that sees nothing (a
-    sequence shorter than its queries) answers zeros.  Returns ``out``, which is made if it is not given.  Not in the
+    sequence shorter than its queries) answers zeros.  Returns ``out``, which is made if it is not given and may be the
+    queries themselves.  Not in the
     reference, whose layers leave attention to the serving engine
     (arctic_inference/vllm/swiftkv/llama_swiftkv.py:617-622 is the write in front of it)."""
     if out is None:

@@ -179,3 +179,16 @@ def test_abi_verify_of_no_request(loaded):
     assert abi_verify(lib, batch=0) == 0
     assert lib.arctic_verify_drafts_workspace_bytes(0, 3, 1000, 2) == 0
     assert lib.arctic_verify_drafts_workspace_bytes(2, 3, 128256, 2) > 0
+
+
+def test_an_expanded_output_is_refused(loaded):
+    args = attention_args()
+    args["out"] = torch.zeros(1, *args["query"].shape[1:], dtype=args["query"].dtype).expand(args["query"].shape)
+    with pytest.raises(RuntimeError, match="out must not be expanded"):
+        ops._IMPLS["paged_attention"](*args.values())
+
+
+def test_abi_verify_of_more_requests_than_a_launch_has_lanes_for(loaded):
+    lib = _native.load()
+    assert abi_verify(lib, batch=1 << 24, most=0, vocab=100, ws_bytes=1 << 62) == 1
+    assert b"too many requests" in lib.arctic_last_error()

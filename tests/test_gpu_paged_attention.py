@@ -256,6 +256,45 @@ def test_scores_that_rise_and_fall_with_the_position(ops, dtype, slope, sign):
     check(ops, c)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("new", [1, 4, 20])
+def test_a_negative_scale_and_none(ops, dtype, new):
+    for scale in (-0.2, 0.0):
+        c = make_attention_case(lengths=[150, 900], new=[new] * 2, heads=4, kv_heads=2, size=64, dtype=dtype, seed=32, device=DEV)
+        c["scale"] = scale
+        check(ops, c)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lengths,new", [([40, 7], 1), ([3000, 900], 3), ([3000, 900], 150)])
+def test_the_output_may_be_the_queries(ops, dtype, lengths, new):
+    c = make_attention_case(lengths=lengths, new=[new] * 2, heads=8, kv_heads=2, size=64, dtype=dtype, seed=33, device=DEV)
+    want = ops.paged_attention_ragged(c["query"], c["query_start"], *cache_args(c))
+    query = c["query"].clone()
+    assert ops.paged_attention_ragged(query, c["query_start"], *cache_args(c), out=query) is query
+    assert torch.equal(query, want)
+    want = ops.paged_attention(c["query"].view(2, new, 8, 64), *cache_args(c))
+    query = c["query"].clone().view(2, new, 8, 64)
+    ops.paged_attention(query, *cache_args(c), out=query)
+    assert torch.equal(query, want)
+
+
+@pytest.mark.parametrize("dtype,size", [(torch.bfloat16, 8), (torch.float32, 5)])
+def test_more_rows_than_a_launch_has_lanes_for(ops, dtype, size):
+    """2.4 million sequences of one token, 8 heads of which a wave or a workgroup answers each: more than 2^32 lanes."""
+    batch, heads = 2_400_001, 8
+    query = torch.ones(batch, heads, size, dtype=dtype, device=DEV)
+    cache = torch.arange(64 * 16 * heads * size, device=DEV).remainder(251).to(dtype).view(64, 16, heads, size)
+    table = torch.arange(batch, device=DEV, dtype=torch.int32).remainder(64)[:, None]
+    lens = torch.ones(batch, dtype=torch.int32, device=DEV)
+    one = torch.ones(1, device=DEV)
+    got = ops.paged_attention(query, cache, cache, table, lens, "auto", one, one, 0.1, 1)
+    assert torch.equal(got, cache[:, 0][table[:, 0].long()])
+    start = torch.arange(batch + 1, dtype=torch.int32, device=DEV)
+    got = ops.paged_attention_ragged(query, start, cache, cache, table, lens, "auto", one, one, 0.1, 1)
+    assert torch.equal(got, cache[:, 0][table[:, 0].long()])
+
+
 def test_no_sequence_and_no_query(ops):
     c = make_attention_case(lengths=[30], new=[1], heads=4, kv_heads=2, size=64, seed=24, device=DEV)
     empty = torch.empty(0, dtype=torch.int32, device=DEV)
