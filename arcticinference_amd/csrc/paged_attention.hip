@@ -271,9 +271,9 @@ static bool few_shape(FewShape &f, int64_t batch, int64_t new_tokens, int num_he
   f.row_tiles = (int)row_tiles;
   const int64_t tiles = most_tiles(max_seq_len, new_tokens, window, num_sinks), units = (c.num_kv_heads / f.heads) * row_tiles;
   // Two workgroups for every CU, all alike, read at the rate that a large read reaches; four lose 5 to 10 % (64 sequences of
-  // 2048 to 8192 keys, 8 heads x 128: fp8 136 us / 152, bf16 259 / 273); of four tiles at least (one of 777 keys: 9.8 us, with
-  // eight 10.2).  Sequences of few tiles are not worth the join, and what few are depends on the CUs that would idle.  Whole /
-  // dealt, 32 heads over 8, us: 16 of 1000 keys (128 workgroups) 17.2 / 19.8, of 777 15.6 / 20.7; 4 of 1000 15.0 / 11.4;
+  // 2048 to 8192 keys, 8 heads x 128: fp8 136 us / 152, bf16 259 / 273).  A piece has four tiles at least (one sequence of 777
+  // keys: 9.8 us, with eight 10.2).  Sequences of few tiles are not worth the join; how many that is depends on the CUs that
+  // would idle.  Whole / dealt, 32 heads over 8, us: 16 of 1000 keys (128 workgroups) 17.2 / 19.8, of 777 15.6 / 20.7; 4 of 1000 15.0 / 11.4;
   // 32 of 1500 (256 workgroups) 33.3 / 40.6, fp8 64 of 1500 34.8 / 41.2; 4 of 1500 19.1 / 15.2.
   constexpr int64_t kWorkgroups = 512, kLeast = 4;
   const int64_t whole = batch * units >= 256 ? 64 : batch * units >= 128 ? 32 : 16;

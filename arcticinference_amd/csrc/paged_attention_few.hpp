@@ -15,7 +15,7 @@
 // bits, so that the rounding of a weight that stands alone cancels, and it needs no exchange between lanes.
 //
 // Heads of 128, 32 over 8: 64 sequences of up to 8192 fp8 keys 130 us, 5.0 TB/s; 3 of up to 131072 16-bit keys 242 us,
-// 5.5 TB/s; one of 777 keys 11 us, 8.6 of them here (memory latencies in a row) and 3.2 in the join.
+// 5.5 TB/s; one of 777 keys 10.6 us, 8.1 of them here (memory latencies in a row) and 3.4 in the join.
 #pragma once
 
 #include "paged_attention.hpp"
