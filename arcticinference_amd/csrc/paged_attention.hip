@@ -282,7 +282,7 @@ static bool few_shape(FewShape &f, int64_t batch, int64_t new_tokens, int num_he
     f.least = 0;
   } else {
     f.least = (int)kLeast;
-    f.workers = (int)std::max<int64_t>(1, std::min((kWorkgroups + units - 1) / units, (batch * tiles + kLeast - 1) / kLeast));
+    f.workers = (int)std::max<int64_t>(1, std::min((kWorkgroups + units - 1) / units, batch * ((tiles + kLeast - 1) / kLeast)));
   }
   // fewer than 2^32 lanes in either launch (a wave joins a row)
   return units * f.workers <= 0xffffffLL && batch * new_tokens * num_heads <= 0x3ffffffLL;

@@ -140,13 +140,15 @@ struct Tiles {
 // How the sequences' tiles, one sequence behind the other, are dealt out: found by every wave for itself.
 struct Deal {
   int64_t at, stop;   // a worker's tiles
-  int64_t begin;      // the first tile of sequence b, which tile `at` belongs to
+  int64_t begin;      // the first tile of sequence b, which tile `at` belongs to (a multiple of `per` where shares are of one
+                      // sequence each: the last one's tiles that there are not count too)
   int64_t per;        // tiles of a worker
   int b;
-  __device__ __forceinline__ static int64_t up_to(int64_t v, int lane) {
+  template <typename I>
+  __device__ __forceinline__ static I up_to(I v, int lane) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-      const int64_t other = __shfl_up(v, d);
+      const I other = __shfl_up(v, d);
       if (lane >= d) v += other;
     }
     return v;
@@ -156,7 +158,7 @@ struct Deal {
     const int lane = threadIdx.x & 63;
     auto count = [&](int i) { return i < p.batch ? Tiles(p, clamped_length(p, i), p.new_tokens).count : 0; };
     const int n = count(lane);
-    const int64_t upto = up_to(n, lane);
+    const int64_t upto = up_to((int64_t)n, lane);
     int64_t total = __shfl(upto, 63);
     if (p.batch > 64) {
       int64_t rest = 0;
@@ -164,6 +166,24 @@ struct Deal {
       total += __shfl(up_to(rest, lane), 63);
     }
     per = max((int64_t)fp.least, (total + fp.workers - 1) / fp.workers);
+    // A worker whose tiles are of two sequences does everything but reading them twice.  Where shares are small that is much,
+    // and no worker does if every sequence begins with one, for which shares an eighth or a quarter larger may do.
+    if (p.batch > 1 && p.batch <= 64 && per <= 64) {
+      for (int grown = 0; grown < 3; ++grown) {
+        const uint32_t share = ((uint32_t)per * (8 + grown) + 7) / 8;
+        const int pieces = (int)(((uint32_t)n + share - 1) / share), last = up_to(pieces, lane);
+        if (__shfl(last, 63) > fp.workers) continue;
+        per = share;
+        at = (int64_t)worker * per;
+        stop = b = 0;
+        const uint64_t beyond = __ballot(last > worker);
+        if (!beyond) return;
+        b = __builtin_ctzll(beyond);
+        begin = (int64_t)__shfl(last - pieces, b) * per;
+        stop = min(at + per, begin + __shfl(n, b));
+        return;
+      }
+    }
     at = (int64_t)worker * per;
     stop = min(total, at + per);
     b = 0;
@@ -172,7 +192,7 @@ struct Deal {
     int64_t before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
       const int own = b0 ? count(b0 + lane) : n;
-      const int64_t now = before + (b0 ? up_to(own, lane) : upto);
+      const int64_t now = before + (b0 ? up_to((int64_t)own, lane) : upto);
       const uint64_t beyond = __ballot(now > at);
       if (beyond) {
         const int l = __builtin_ctzll(beyond);
