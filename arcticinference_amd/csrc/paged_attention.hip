@@ -273,8 +273,8 @@ static bool few_shape(FewShape &f, int64_t batch, int64_t new_tokens, int num_he
   // Two workgroups for every CU, all alike, read at the rate that a large read reaches; four lose 5 to 10 % (64 sequences of
   // 2048 to 8192 keys, 8 heads x 128: fp8 136 us / 152, bf16 259 / 273).  A piece has four tiles at least (one sequence of 777
   // keys: 9.8 us, with eight 10.2).  Sequences of few tiles are not worth the join; how many that is depends on the CUs that
-  // would idle.  Whole / dealt, 32 heads over 8, us: 16 of 1000 keys (128 workgroups) 17.2 / 19.8, of 777 15.6 / 20.7; 4 of 1000 15.0 / 11.4;
-  // 32 of 1500 (256 workgroups) 33.3 / 40.6, fp8 64 of 1500 34.8 / 41.2; 4 of 1500 19.1 / 15.2.
+  // would idle.  Whole / dealt, 32 heads over 8, us: 16 of 1000 keys (128 workgroups) 17.2 / 20.1, of 777 15.6 / 16.8; 4 of
+  // 1000 15.0 / 10.9; 32 of 1500 (256 workgroups) 33.3 / 37.7, fp8 64 of 1500 34.8 / 40.7; 4 of 1500 19.1 / 12.6.
   constexpr int64_t kWorkgroups = 512, kLeast = 4;
   const int64_t whole = batch * units >= 256 ? 64 : batch * units >= 128 ? 32 : 16;
   if (tiles <= whole) {

@@ -232,6 +232,17 @@ def test_few_long_sequences(ops, kv):
     check(ops, make_attention_case(lengths=[9001], new=[40], heads=4, kv_heads=1, size=64, kv=kv, seed=22, device=DEV))
 
 
+@pytest.mark.parametrize("batch", [2, 5, 16, 40, 64, 65])
+@pytest.mark.parametrize("longest", [600, 1500, 4000])
+def test_tiles_dealt_to_workers(ops, batch, longest):
+    """Sequences of equal and of very unequal lengths, so that shares fit as they are, fit when they grow, and do not."""
+    g = torch.Generator().manual_seed(batch * longest)
+    unequal = [longest] + torch.randint(1, longest, (batch - 1,), generator=g).tolist()
+    for lengths in ([longest] * batch, unequal, [longest] + [1] * (batch - 1)):
+        c = make_attention_case(lengths=lengths, new=[1] * batch, heads=4, kv_heads=2, size=64, seed=34, device=DEV)
+        check(ops, c, ragged=False)
+
+
 def test_a_peak_in_any_split(ops):
     """One key holds nearly all the weight: first, last, in the middle."""
     for at in (0, 2500, 4999):
